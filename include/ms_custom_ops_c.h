@@ -213,6 +213,72 @@ int ms_custom_ops_fa_update_infer(const MsTensorDesc *lse, const MsTensorDesc *l
 int ms_custom_ops_fa_update(const MsTensorDesc *lse, const MsTensorDesc *local_out, int64_t fa_update_type,
                             int64_t sp, const MsTensorDesc *output, void *stream);
 
+/* rope_and_cache (extension; formulas at msco_rope_and_cache).  query (tokens, q_heads, head_dim), key and
+ * value (tokens, kv_heads, head_dim), Float16 / BFloat16: the heads of a token must be adjacent, the distance of
+ * two tokens is free (slices of a fused projection).  slot_mapping and positions Int32 (tokens); cos_sin Float32
+ * (max_positions, rotary_dim); q_weight / k_weight (head_dim) or NULL; caches (num_blocks, block_size, kv_heads,
+ * head_dim) for input_layout 0, (num_blocks, kv_heads, block_size, head_dim) for 1, of key's type or -- with k_descale /
+ * v_descale Float32 and optional k_offset / v_offset Int32, (kv_heads * head_dim) -- Int8.  query_out: caller-allocated,
+ * contiguous, query's shape and dtype.  oob_count: Int32 (1) or NULL; incremented per dropped token.
+ * `_infer` does the checks and gives query_out's dtype and shape. */
+int ms_custom_ops_rope_and_cache_infer(const MsTensorDesc *query, const MsTensorDesc *key, const MsTensorDesc *value,
+                                       const MsTensorDesc *key_cache, const MsTensorDesc *value_cache,
+                                       const MsTensorDesc *slot_mapping, const MsTensorDesc *positions,
+                                       const MsTensorDesc *cos_sin, const MsTensorDesc *q_weight,
+                                       const MsTensorDesc *k_weight, double eps, int32_t interleaved,
+                                       int64_t input_layout, const MsTensorDesc *k_descale,
+                                       const MsTensorDesc *k_offset, const MsTensorDesc *v_descale,
+                                       const MsTensorDesc *v_offset, const MsTensorDesc *oob_count,
+                                       int32_t *out_dtype, int32_t *out_ndim, int64_t *out_shape /* [MS_MAX_DIMS] */);
+int ms_custom_ops_rope_and_cache(const MsTensorDesc *query, const MsTensorDesc *key, const MsTensorDesc *value,
+                                 const MsTensorDesc *key_cache, const MsTensorDesc *value_cache,
+                                 const MsTensorDesc *slot_mapping, const MsTensorDesc *positions,
+                                 const MsTensorDesc *cos_sin, const MsTensorDesc *q_weight,
+                                 const MsTensorDesc *k_weight, double eps, int32_t interleaved, int64_t input_layout,
+                                 const MsTensorDesc *k_descale, const MsTensorDesc *k_offset,
+                                 const MsTensorDesc *v_descale, const MsTensorDesc *v_offset,
+                                 const MsTensorDesc *oob_count, const MsTensorDesc *query_out, void *stream);
+
+/* chunk_attention (extension; formulas at msco_chunk_attention).  query (tokens, q_heads, head_dim); caches and
+ * input_layout as above; block_tables Int32 (sequences, max_blocks); q_seq_lens and context_lens Int32 (sequences)
+ * on the HOST, with sum(q_seq_lens) <= tokens; scales and offsets as above.  out: caller-allocated, query's shape and
+ * dtype, its rows behind the last sequence's are left as they are; lse: Float32 (tokens, q_heads) or NULL.
+ * `_workspace_size` plans only (no device work); `workspace` is 256-byte aligned device memory of that size. */
+typedef struct MsChunkAttentionArgs {
+  const MsTensorDesc *query;
+  const MsTensorDesc *key_cache;
+  const MsTensorDesc *value_cache;
+  const MsTensorDesc *block_tables;
+  const MsTensorDesc *q_seq_lens;   /* int32, on host */
+  const MsTensorDesc *context_lens; /* int32, on host */
+  const MsTensorDesc *k_descale;
+  const MsTensorDesc *k_offset;
+  const MsTensorDesc *v_descale;
+  const MsTensorDesc *v_offset;
+  const MsTensorDesc *oob_count;
+  double qk_scale;
+  int64_t window_size;
+  int64_t input_layout;
+} MsChunkAttentionArgs;
+int ms_custom_ops_chunk_attention_infer(const MsChunkAttentionArgs *args, int32_t *out_dtype, int32_t *out_ndim,
+                                        int64_t *out_shape /* [MS_MAX_DIMS] */);
+int ms_custom_ops_chunk_attention_workspace_size(const MsChunkAttentionArgs *args, size_t *bytes);
+int ms_custom_ops_chunk_attention(const MsChunkAttentionArgs *args, const MsTensorDesc *out, const MsTensorDesc *lse,
+                                  void *workspace, size_t workspace_bytes, void *stream);
+
+/* verify_draft_tokens (extension; rule at msco_verify_draft_tokens).  target_probs (batch, drafts + 1, vocab),
+ * draft_probs (batch, drafts, vocab) or NULL, Float32 / Float16 / BFloat16; draft_tokens Int32 (batch, drafts);
+ * uniform Float32 (batch, drafts + 1); draft_lens Int32 (batch) or NULL.  tokens Int32 (batch, drafts + 1) and
+ * accepted Int32 (batch) are caller-allocated.  `_infer` does the checks and gives tokens' shape. */
+int ms_custom_ops_verify_draft_tokens_infer(const MsTensorDesc *target_probs, const MsTensorDesc *draft_probs,
+                                            const MsTensorDesc *draft_tokens, const MsTensorDesc *uniform,
+                                            const MsTensorDesc *draft_lens, int32_t *out_dtype, int32_t *out_ndim,
+                                            int64_t *out_shape /* [MS_MAX_DIMS] */);
+int ms_custom_ops_verify_draft_tokens(const MsTensorDesc *target_probs, const MsTensorDesc *draft_probs,
+                                      const MsTensorDesc *draft_tokens, const MsTensorDesc *uniform,
+                                      const MsTensorDesc *draft_lens, const MsTensorDesc *tokens,
+                                      const MsTensorDesc *accepted, void *stream);
+
 const char *ms_custom_ops_last_error(void);
 int ms_custom_ops_last_error_kind(void);
 

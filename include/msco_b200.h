@@ -421,6 +421,94 @@ int msco_decode_step_gather(const MscoPaPlan *plan, const void *key, const void 
                             const void *attn_mask, void *out, void *workspace, size_t workspace_bytes,
                             void *stream, const MscoGatherDesc *gather, uint32_t step);
 
+/* ------------------------------------------------------------------------
+ * rope_and_cache (extension): what stands in front of the cache write of a serving step, in one pass.
+ * Per token t and head row x (head_dim elements) of query and key:
+ *     n_d = x_d * w_d / sqrt(mean(x^2) + eps)           only with a weight (q_weight / k_weight, may be NULL)
+ *     (a, b) -> (a c_i - b s_i, b c_i + a s_i)          for the pairs i < rotary_dim / 2,
+ * with (a, b) = (n_i, n_{i + rotary_dim/2}), or (n_2i, n_{2i+1}) when interleaved, c_i / s_i =
+ * cos_sin[positions[t]][i] / [rotary_dim/2 + i]; elements from rotary_dim on pass through.  All in float32,
+ * rounded once.  Rotated queries go to query_out [tokens, q_heads, head_dim]; rotated keys and the values
+ * as they are go to row slot_mapping[t] of the caches (negative slots: no cache write), as 16-bit rows or --
+ * int8 caches -- quantised per channel like msco_reshape_and_cache_quant (from the float32 value).
+ * query / key / value rows may be slices of a fused projection: *_stride is the distance of two tokens in
+ * elements, heads of a token are adjacent.  Slots >= num_blocks * block_size are dropped; a token whose position
+ * is outside [0, max_positions) is written as zeros to query_out and not to the caches; both are counted in
+ * *oob_count (device int32, may be NULL).
+ * ---------------------------------------------------------------------- */
+typedef struct MscoRopeDesc {
+  int32_t dtype;                     /* query / key / value / query_out / weights: F16 or BF16   */
+  int32_t cache_dtype;               /* the same type, or I8                                     */
+  int32_t num_q_heads, num_kv_heads; /* num_q_heads may be 0 (keys and values only)              */
+  int32_t head_dim, rotary_dim;      /* head_dim <= 512; rotary_dim even, <= head_dim            */
+  int32_t block_size, cache_layout;  /* 0: [blocks, block_size, kv_heads, head_dim], 1: [blocks, kv_heads, block_size, head_dim] */
+  int64_t num_blocks;
+  int64_t num_tokens;
+  int64_t max_positions;             /* rows of cos_sin                                          */
+  int64_t q_stride, k_stride, v_stride;
+  float eps;
+  int32_t interleaved;
+} MscoRopeDesc;
+int msco_rope_and_cache(const MscoRopeDesc *desc, const void *query, const void *key, const void *value,
+                        void *query_out, void *key_cache, void *value_cache, const int32_t *slot_mapping,
+                        const int32_t *positions, const float *cos_sin, const void *q_weight,
+                        const void *k_weight, const float *k_descale, const int32_t *k_offset,
+                        const float *v_descale, const int32_t *v_offset, int32_t *oob_count, void *stream);
+
+/* ------------------------------------------------------------------------
+ * chunk_attention (extension): causal attention of a chunk of new tokens per sequence over the paged cache,
+ * which already holds the new tokens' keys and values.  Sequence b has q_len = host_q_seq_lens[b] >= 0 new
+ * tokens and ctx = host_context_lens[b] >= 0 cached ones; its i-th new token stands at position
+ * ctx - q_len + i and sees the cached tokens j with position - window < j <= position (window 0: all of
+ * them up to its position).  A token that sees nothing gives zeros (lse -inf).
+ *   query / out  [tokens, num_q_heads, head_dim], the sequences' tokens one after the other; rows behind the
+ *                last sequence's are neither read as queries nor written
+ *   caches       as in msco_paged_attention_launch (both layouts; int8 with descale / offset per channel)
+ *   lse          float32 [tokens, num_q_heads] or NULL
+ * Lengths are read on the host during the call; nothing of them is kept.  Block ids outside the cache are read
+ * as block 0 and counted in *oob_count (device int32, may be NULL).  Cached tokens that no query of the chunk
+ * may see are not read, or do not count whatever they hold.  The result of a sequence does not depend on
+ * the other sequences of the call.
+ * `workspace`: 256-byte aligned device memory of msco_chunk_attention_workspace bytes (may be 0), not
+ * shared with a call in flight; it needs no initialisation.
+ * ---------------------------------------------------------------------- */
+typedef struct MscoChunkDesc {
+  int32_t q_dtype, kv_dtype;         /* F16 / BF16; the cache the same, or I8                    */
+  int32_t num_q_heads, num_kv_heads, head_dim, block_size;
+  int64_t num_blocks;
+  int32_t max_blocks_per_seq;
+  int32_t cache_layout;
+  float qk_scale;
+  int32_t window;                    /* 0: none                                                  */
+  int32_t kernel;                    /* 0: by the shape, 1: the general kernel                   */
+  int32_t reserved;
+} MscoChunkDesc;
+int msco_chunk_attention_workspace(const MscoChunkDesc *desc, const int32_t *host_q_seq_lens,
+                                   const int32_t *host_context_lens, int32_t batch, size_t *bytes);
+int msco_chunk_attention(const MscoChunkDesc *desc, const int32_t *host_q_seq_lens,
+                         const int32_t *host_context_lens, int32_t batch, const void *query,
+                         const void *key_cache, const void *value_cache, const int32_t *block_tables,
+                         const float *k_descale, const int32_t *k_offset, const float *v_descale,
+                         const int32_t *v_offset, void *out, float *lse, void *workspace,
+                         size_t workspace_bytes, int32_t *oob_count, void *stream);
+
+/* ------------------------------------------------------------------------
+ * verify_draft_tokens (extension): rejection sampling of drafted tokens against the target's probabilities.
+ *   target_probs [batch, drafts + 1, vocab], draft_probs [batch, drafts, vocab] (F32 / F16 / BF16, the same type) or
+ *   NULL (the drafts were certain: probability 1); draft_tokens int32 [batch, drafts]; draft_lens int32 [batch]
+ *   or NULL (all `drafts`), clamped to [0, drafts]; uniform float32 [batch, drafts + 1] in [0, 1)
+ * Draft i of a row is accepted while uniform[i] * draft(token) < target(token) (products in 64 bits; a token id
+ * outside the vocabulary is turned down).  At the first draft n that is not, a token is drawn from
+ * max(target[n] - draft[n], 0) (from target[n] where that is nowhere positive); when all are accepted, from
+ * target[n].  The draw is the lowest t with sum(weights[0..t]) > uniform[drafts] * sum(weights), sums in 64 bits.
+ *   tokens int32 [batch, drafts + 1]: the accepted drafts, the drawn token, -1 behind it (the drawn token is
+ *   -1 where target[n] is nowhere positive); accepted int32 [batch]
+ * ---------------------------------------------------------------------- */
+int msco_verify_draft_tokens(const void *target_probs, const void *draft_probs, int32_t dtype,
+                             const int32_t *draft_tokens, const int32_t *draft_lens, const float *uniform,
+                             int32_t *tokens, int32_t *accepted, int32_t batch, int32_t drafts, int32_t vocab,
+                             void *stream);
+
 /* Kernel timing for benchmarks.  After msco_paged_attention_profile_enable(plan, 1) every launch
  * of this plan records a pair of CUDA events directly around the attention kernel (not around the
  * plan upload or the reduce kernel) into a ring of 64 pairs owned by the plan.

@@ -1,5 +1,6 @@
 """B200-native paged-KV decode operators: ``reshape_and_cache`` and ``paged_attention``, with the
-two operators either side of them, ``paged_cache_load`` and ``fa_update``.
+two operators either side of them, ``paged_cache_load`` and ``fa_update``, and the operators of a step that
+brings more than one token per sequence: ``rope_and_cache``, ``chunk_attention`` and ``verify_draft_tokens``.
 
 Drop-in for the operators of the same names in ``ms_custom_ops``
 (python/ms_custom_ops/__init__.py:76 re-exports them from the plugin module;
@@ -19,6 +20,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import struct
 import threading
 import weakref
 
@@ -33,7 +35,9 @@ __all__ = ["reshape_and_cache", "reshape_and_cache_infer", "reshape_and_cache_np
            "reshape_and_cache_quant", "paged_attention",
            "paged_attention_infer", "plan_arena_stats",
            "paged_cache_load", "paged_cache_load_infer", "fa_update", "fa_update_infer", "paged_attention_with_lse",
-           "paged_attention_workspace_size", "paged_attention_check_status", "TensorSpec", "MscoError",
+           "paged_attention_workspace_size", "paged_attention_check_status", "rope_and_cache", "rope_and_cache_infer",
+           "chunk_attention", "chunk_attention_infer", "chunk_attention_workspace_size", "verify_draft_tokens",
+           "verify_draft_tokens_infer", "TensorSpec", "MscoError",
            "UnsupportedOnB200", "registered_ops", "plan_cache_stats", "plan_cache_clear"]
 
 _DT = {"float16": _abi.DTYPE_F16, "bfloat16": _abi.DTYPE_BF16, "int8": _abi.DTYPE_I8,
@@ -486,6 +490,269 @@ def fa_update(lse, local_out, fa_update_type=0, sp=1):
     _host.check(_host.lib().ms_custom_ops_fa_update(D(lse), D(local_out), int(fa_update_type), int(sp), D(out),
                                                     _stream()))
     return out
+
+
+# --------------------------------------------------------------------------
+# operators of a step with more than one token per sequence
+# --------------------------------------------------------------------------
+_DESC_STRUCT = struct.Struct(f"Pii{_host.MS_MAX_DIMS}q{_host.MS_MAX_DIMS}qii")
+assert _DESC_STRUCT.size == C.sizeof(_host.MsTensorDesc)
+_DESC_SLOTS = 24
+_PADS = tuple((0,) * (_host.MS_MAX_DIMS - n) for n in range(_host.MS_MAX_DIMS + 1))
+_torch_codes = {}  # torch.dtype -> MSCO_DTYPE_*
+
+
+class _Packer:
+    """Tensor descriptors of one call, written into a buffer that the thread keeps (one struct.pack_into per
+    tensor).  Checks that all device tensors are on the first one's device."""
+
+    def __init__(self):
+        self.array = (_host.MsTensorDesc * _DESC_SLOTS)()
+        self.ptrs = [C.pointer(self.array[i]) for i in range(_DESC_SLOTS)]
+        self.size = C.sizeof(_host.MsTensorDesc)
+        self.keep = []
+        self.used = 0
+        self.device = -1
+        self.chunk_args = _host.MsChunkAttentionArgs()
+
+    def start(self, device):
+        self.used = 0
+        self.device = device
+        self.keep.clear()
+        return self
+
+    def __call__(self, t, host=False):
+        if t is None:
+            return None
+        if host and isinstance(t, (list, tuple, np.ndarray)):
+            a = np.asarray(t)
+            a = np.ascontiguousarray(a.astype(np.int32) if isinstance(t, (list, tuple)) else a)
+            self.keep.append(a)
+            values = (a.ctypes.data, _dtype_code(str(a.dtype)), a.ndim, a.shape, _contig_strides(a.shape), 1)
+        else:
+            try:
+                at = t.get_device()
+            except AttributeError:
+                raise TypeError("device tensors must be torch CUDA tensors") from None
+            if at < 0:
+                if t.numel() and not host:
+                    raise RuntimeError("the operator takes CUDA tensors (only lengths are read on the host)")
+            elif at != self.device:
+                raise RuntimeError(f"all tensors must be on one device, got cuda:{self.device} and cuda:{at}")
+            code = _torch_codes.get(t.dtype)
+            if code is None:
+                code = _torch_codes[t.dtype] = _dtype_code(t.dtype)
+            values = (t.data_ptr(), code, t.dim(), t.shape, t.stride(), 1 if at < 0 else 0)
+        ptr, code, n, shape, strides, on_host = values
+        if n > _host.MS_MAX_DIMS:
+            raise ValueError("tensors of more than 8 dimensions are not supported")
+        i = self.used
+        self.used = i + 1
+        pad = _PADS[n]
+        _DESC_STRUCT.pack_into(self.array, i * self.size, ptr, code, n, *shape, *pad, *strides, *pad, on_host, 0)
+        return self.ptrs[i]
+
+
+def _packer(t):
+    """The thread's packer, for a call on the device of tensor `t`."""
+    try:
+        device = t.get_device()
+    except AttributeError:
+        raise TypeError("device tensors must be torch CUDA tensors") from None
+    if device < 0:
+        raise RuntimeError("the operator takes CUDA tensors (only lengths are read on the host)")
+    p = _tls.__dict__.get("packer")
+    if p is None:
+        p = _tls.packer = _Packer()
+    return p.start(device)
+
+
+def _on_device(device, call):
+    """Runs `call(stream)` with `device` current, on torch's current stream of that device."""
+    import torch
+    if torch.cuda.current_device() == device:
+        return call(torch._C._cuda_getCurrentRawStream(device))
+    with torch.cuda.device(device):
+        return call(torch._C._cuda_getCurrentRawStream(device))
+
+
+def rope_and_cache(query, key, value, key_cache, value_cache, slot_mapping, positions, cos_sin, q_weight=None,
+                   k_weight=None, eps=1e-06, interleaved=False, input_layout=0, k_descale=None, k_offset=None,
+                   v_descale=None, v_offset=None, oob_count=None):
+    """Norm and rotate the queries and keys of a step's tokens and write keys and values to the paged caches;
+    returns the rotated queries (extension: ``reshape_and_cache`` with what stands in front of it).
+
+    query        [tokens, q_heads, head_dim], key / value [tokens, kv_heads, head_dim]; fp16 / bf16.  The heads of a
+                 token must be adjacent; tokens may lie apart (slices of a fused projection)
+    key_cache / value_cache  [num_blocks, block_size, kv_heads, head_dim], or with input_layout = 1
+                 [num_blocks, kv_heads, block_size, head_dim]; the rows' dtype, or int8 with k_descale / v_descale
+                 float32 and optional k_offset / v_offset int32, [kv_heads * head_dim]
+    slot_mapping int32 [tokens]; negative: the token is rotated but not cached
+    positions    int32 [tokens], rows of cos_sin
+    cos_sin      float32 [max_positions, rotary_dim]: the cosines, then the sines, of rotary_dim / 2 angles; elements
+                 of a head from rotary_dim on pass unrotated.  Pairs are (i, i + rotary_dim / 2), or (2i, 2i + 1)
+                 when `interleaved`
+    q_weight / k_weight  [head_dim] or None: RMS norm of every head row over head_dim first
+    oob_count    int32 [1] or None: incremented for every token that is dropped because its slot is behind the
+                 caches or its position outside the table (its row of the result is zero in the latter case)
+    Arithmetic in float32, rounded once.  Two tokens of a call must not have the same slot; the result must not
+    share memory with the inputs (it is a new tensor).
+    """
+    import torch
+    D = _packer(query)
+    out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+    args = (D(query), D(key), D(value), D(key_cache), D(value_cache), D(slot_mapping), D(positions), D(cos_sin),
+            D(q_weight), D(k_weight), float(eps), int(bool(interleaved)), int(input_layout), D(k_descale), D(k_offset),
+            D(v_descale), D(v_offset), D(oob_count), D(out))
+    rc = _on_device(D.device, lambda stream: _host.lib().ms_custom_ops_rope_and_cache(*args, stream))
+    if rc:
+        _host.check(rc)
+    return out
+
+
+def rope_and_cache_infer(query, key, value, key_cache, value_cache, slot_mapping, positions, cos_sin, q_weight=None,
+                         k_weight=None, eps=1e-06, interleaved=False, input_layout=0, k_descale=None, k_offset=None,
+                         v_descale=None, v_offset=None, oob_count=None):
+    """Shape and dtype of the rotated queries after the operator's checks; TensorSpec or real tensors."""
+    D = _Descs()
+    dt, nd, shp = C.c_int32(), C.c_int32(), (C.c_int64 * _host.MS_MAX_DIMS)()
+    _host.check(_host.lib().ms_custom_ops_rope_and_cache_infer(
+        D(query), D(key), D(value), D(key_cache), D(value_cache), D(slot_mapping), D(positions), D(cos_sin),
+        D(q_weight), D(k_weight), float(eps), int(bool(interleaved)), int(input_layout), D(k_descale), D(k_offset),
+        D(v_descale), D(v_offset), D(oob_count), C.byref(dt), C.byref(nd), shp))
+    return tuple(shp[i] for i in range(nd.value)), _DT_NAMES[dt.value]
+
+
+def _chunk_args(a, D, query, key_cache, value_cache, block_tables, q_seq_lens, context_lens, qk_scale, window_size,
+                input_layout, k_descale, k_offset, v_descale, v_offset, oob_count, host):
+    a.query, a.key_cache, a.value_cache = D(query), D(key_cache), D(value_cache)
+    a.block_tables = D(block_tables)
+    a.q_seq_lens, a.context_lens = D(q_seq_lens, **host), D(context_lens, **host)
+    a.k_descale, a.k_offset, a.v_descale, a.v_offset = D(k_descale), D(k_offset), D(v_descale), D(v_offset)
+    a.oob_count = D(oob_count)
+    a.qk_scale, a.window_size, a.input_layout = float(qk_scale), int(window_size), int(input_layout)
+    return a
+
+
+def chunk_attention(query, key_cache, value_cache, block_tables, q_seq_lens, context_lens, qk_scale=1.0, window_size=0,
+                    input_layout=0, k_descale=None, k_offset=None, v_descale=None, v_offset=None, out=None,
+                    return_lse=False, oob_count=None):
+    """Causal attention of a chunk of new tokens per sequence over the paged KV cache (extension: chunked prefill,
+    speculative tokens and single tokens in one ragged batch); returns ``attention_out`` shaped like `query`.
+
+    query        [tokens, q_heads, head_dim] fp16 / bf16: the new tokens of the sequences one after the other
+    key_cache / value_cache  as in ``paged_attention`` (input_layout 0 or 1; int8 with k_descale / v_descale and
+                 optional offsets); they hold the new tokens' keys and values already (``rope_and_cache``)
+    block_tables int32 [sequences, max_blocks]
+    q_seq_lens   int32 [sequences] on the HOST: new tokens of each sequence, 0 allowed
+    context_lens int32 [sequences] on the HOST: cached tokens, the new ones included
+    window_size  a token sees the last `window_size` positions up to its own; 0: all of them
+    out          where to write (contiguous, query's shape and dtype, not query's memory); rows behind the last
+                 sequence's are left as they are.  Without it a new tensor is returned, those rows zero
+    return_lse   also return float32 [tokens, q_heads]: log of the sum of exp(qk_scale * q.k), as
+                 ``paged_attention_with_lse`` does (-inf where a token sees nothing, and in the rows behind)
+    oob_count    int32 [1] or None: incremented for every block id outside the cache that was met (such a block
+                 is read as block 0)
+    The i-th of q_len new tokens stands at position context_len - q_len + i; one that sees nothing gives zeros.
+    The lengths are read during the call: a captured graph replays with the lengths it was captured with.
+    """
+    import torch
+    D = _packer(query)
+    device, tokens = query.device, query.shape[0]
+    if out is None:
+        out = torch.empty(query.shape, dtype=query.dtype, device=device)
+        fill = True
+    else:
+        fill = False
+    lse = torch.empty(query.shape[:2], dtype=torch.float32, device=device) if return_lse else None
+    a = _chunk_args(D.chunk_args, D, query, key_cache, value_cache, block_tables, q_seq_lens, context_lens, qk_scale,
+                    window_size, input_layout, k_descale, k_offset, v_descale, v_offset, oob_count, {"host": True})
+    out_desc, lse_desc = D(out), D(lse)
+    L = _host.lib()
+    need = C.c_size_t()
+    rc = L.ms_custom_ops_chunk_attention_workspace_size(C.byref(a), C.byref(need))
+    if rc:
+        _host.check(rc)
+    # from the allocator, per call: it belongs to this call's stream, or to the graph that is being captured
+    ws = torch.empty(need.value, dtype=torch.uint8, device=device) if need.value else None
+    rc = _on_device(D.device, lambda stream: L.ms_custom_ops_chunk_attention(
+        C.byref(a), out_desc, lse_desc, None if ws is None else ws.data_ptr(), need.value, stream))
+    if rc:
+        _host.check(rc)
+    if fill or return_lse:
+        rows = int(np.sum(np.asarray(q_seq_lens), dtype=np.int64))
+        if rows < tokens:
+            if fill:
+                out[rows:].zero_()
+            if return_lse:
+                lse[rows:].fill_(-math.inf)
+    return (out, lse) if return_lse else out
+
+
+def chunk_attention_infer(query, key_cache, value_cache, block_tables, q_seq_lens, context_lens, qk_scale=1.0,
+                          window_size=0, input_layout=0, k_descale=None, k_offset=None, v_descale=None, v_offset=None,
+                          oob_count=None):
+    """Shape and dtype of the output after the operator's checks; TensorSpec or real tensors (lengths with values)."""
+    D = _Descs()
+    a = _chunk_args(_host.MsChunkAttentionArgs(), D, query, key_cache, value_cache, block_tables, q_seq_lens,
+                    context_lens, qk_scale, window_size, input_layout, k_descale, k_offset, v_descale, v_offset,
+                    oob_count, {"host_ok": True})
+    dt, nd, shp = C.c_int32(), C.c_int32(), (C.c_int64 * _host.MS_MAX_DIMS)()
+    _host.check(_host.lib().ms_custom_ops_chunk_attention_infer(C.byref(a), C.byref(dt), C.byref(nd), shp))
+    return tuple(shp[i] for i in range(nd.value)), _DT_NAMES[dt.value]
+
+
+def chunk_attention_workspace_size(query, key_cache, value_cache, block_tables, q_seq_lens, context_lens, qk_scale=1.0,
+                                   window_size=0, input_layout=0, k_descale=None, k_offset=None, v_descale=None,
+                                   v_offset=None) -> int:
+    """Bytes of device workspace a launch with these arguments needs (planning only, no GPU work)."""
+    D = _Descs()
+    a = _chunk_args(_host.MsChunkAttentionArgs(), D, query, key_cache, value_cache, block_tables, q_seq_lens,
+                    context_lens, qk_scale, window_size, input_layout, k_descale, k_offset, v_descale, v_offset, None,
+                    {"host_ok": True})
+    n = C.c_size_t()
+    _host.check(_host.lib().ms_custom_ops_chunk_attention_workspace_size(C.byref(a), C.byref(n)))
+    return int(n.value)
+
+
+def verify_draft_tokens(target_probs, draft_probs, draft_tokens, uniform, draft_lens=None):
+    """Rejection sampling of drafted tokens against the target's probabilities; returns ``(tokens, accepted)``
+    (extension: what follows the multi-token attention of a speculative step).
+
+    target_probs [batch, drafts + 1, vocab] fp32 / fp16 / bf16: the target's distribution at every draft, and after
+                 the last
+    draft_probs  [batch, drafts, vocab], the same dtype: what the drafts were drawn from; None: they were certain
+    draft_tokens int32 [batch, drafts]
+    uniform      float32 [batch, drafts + 1] in [0, 1): one number per draft, and the last for the drawn token
+    draft_lens   int32 [batch] on the device: drafts of each row (clamped to [0, drafts]); None: all
+    Draft i is accepted while ``uniform[i] * draft_probs[i, token] < target_probs[i, token]``.  At the first that is
+    not, a token is drawn from max(target - draft, 0); when all are accepted, from the target's next distribution:
+    the lowest token whose running sum exceeds ``uniform[:, drafts]`` times the sum of all (64-bit sums).
+    tokens       int32 [batch, drafts + 1]: the accepted drafts, the drawn token, then -1 (the drawn token is -1
+                 where the target is nowhere positive)
+    accepted     int32 [batch]
+    """
+    import torch
+    D = _packer(target_probs)
+    if draft_tokens.dim() != 2:
+        raise ValueError(f"For VerifyDraftTokens, draft_tokens must have rank 2, but got {draft_tokens.dim()}.")
+    batch, drafts = draft_tokens.shape
+    tokens = torch.empty((batch, drafts + 1), dtype=torch.int32, device=target_probs.device)
+    accepted = torch.empty((batch,), dtype=torch.int32, device=target_probs.device)
+    args = (D(target_probs), D(draft_probs), D(draft_tokens), D(uniform), D(draft_lens), D(tokens), D(accepted))
+    rc = _on_device(D.device, lambda stream: _host.lib().ms_custom_ops_verify_draft_tokens(*args, stream))
+    if rc:
+        _host.check(rc)
+    return tokens, accepted
+
+
+def verify_draft_tokens_infer(target_probs, draft_probs, draft_tokens, uniform, draft_lens=None):
+    """Shape and dtype of `tokens` after the operator's checks; TensorSpec or real tensors."""
+    D = _Descs()
+    dt, nd, shp = C.c_int32(), C.c_int32(), (C.c_int64 * _host.MS_MAX_DIMS)()
+    _host.check(_host.lib().ms_custom_ops_verify_draft_tokens_infer(
+        D(target_probs), D(draft_probs), D(draft_tokens), D(uniform), D(draft_lens), C.byref(dt), C.byref(nd), shp))
+    return tuple(shp[i] for i in range(nd.value)), _DT_NAMES[dt.value]
 
 
 def paged_attention_check_status(device=None):

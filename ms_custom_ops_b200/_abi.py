@@ -35,6 +35,20 @@ class MscoPaPlanInfo(C.Structure):
     ]
 
 
+class MscoRopeDesc(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("dtype", "cache_dtype", "num_q_heads", "num_kv_heads", "head_dim", "rotary_dim",
+                                         "block_size", "cache_layout")] + [
+        (n, C.c_int64) for n in ("num_blocks", "num_tokens", "max_positions", "q_stride", "k_stride", "v_stride")] + [
+        ("eps", C.c_float), ("interleaved", C.c_int32)]
+
+
+class MscoChunkDesc(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("q_dtype", "kv_dtype", "num_q_heads", "num_kv_heads", "head_dim",
+                                         "block_size")] + [
+        ("num_blocks", C.c_int64), ("max_blocks_per_seq", C.c_int32), ("cache_layout", C.c_int32),
+        ("qk_scale", C.c_float), ("window", C.c_int32), ("kernel", C.c_int32), ("reserved", C.c_int32)]
+
+
 MAX_PEERS = 8
 IPC_HANDLE_BYTES = 64
 
@@ -66,6 +80,7 @@ EXPORTS = (
     "msco_paged_attention_launch_lse", "msco_expand_rows_i32", "msco_paged_attention_replan", "msco_plan_arena_stats",
     "msco_reshape_and_cache_bnsd", "msco_copy_device", "msco_paged_attention_plan_tokens",
     "msco_paged_attention_replan_tokens", "msco_paged_attention_tma_supported", "msco_paged_cache_load_workspace_bytes", "msco_paged_cache_load", "msco_fa_update", "msco_fa_update_strided",
+    "msco_rope_and_cache", "msco_chunk_attention_workspace", "msco_chunk_attention", "msco_verify_draft_tokens",
 )
 
 
@@ -98,6 +113,14 @@ def lib():
     L.msco_fa_update.argtypes = [vp, vp, vp, i64, i32, i32, vp]
     L.msco_fa_update_strided.restype = C.c_int
     L.msco_fa_update_strided.argtypes = [vp, i64, vp, i64, i32, vp, i64, i32, i32, vp]
+    L.msco_rope_and_cache.restype = C.c_int
+    L.msco_rope_and_cache.argtypes = [C.POINTER(MscoRopeDesc)] + [vp] * 17
+    L.msco_chunk_attention_workspace.restype = C.c_int
+    L.msco_chunk_attention_workspace.argtypes = [C.POINTER(MscoChunkDesc), vp, vp, i32, C.POINTER(sz)]
+    L.msco_chunk_attention.restype = C.c_int
+    L.msco_chunk_attention.argtypes = [C.POINTER(MscoChunkDesc), vp, vp, i32] + [vp] * 11 + [sz, vp, vp]
+    L.msco_verify_draft_tokens.restype = C.c_int
+    L.msco_verify_draft_tokens.argtypes = [vp, vp, i32] + [vp] * 5 + [i32] * 3 + [vp]
     L.msco_paged_attention_split_tokens.restype = i32
     L.msco_paged_attention_split_tokens.argtypes = [i32, i32]
     L.msco_paged_attention_split_tokens_for.restype = i32

@@ -32,6 +32,13 @@ class MsPagedAttentionArgs(C.Structure):
         ("scale_type", C.c_int64), ("input_layout", C.c_int64), ("mla_v_dim", C.c_int64), ("input_format", C.c_int64)]
 
 
+class MsChunkAttentionArgs(C.Structure):
+    _fields_ = [(n, _TP) for n in (
+        "query", "key_cache", "value_cache", "block_tables", "q_seq_lens", "context_lens", "k_descale", "k_offset",
+        "v_descale", "v_offset", "oob_count")] + [
+        ("qk_scale", C.c_double), ("window_size", C.c_int64), ("input_layout", C.c_int64)]
+
+
 # every symbol include/ms_custom_ops_c.h declares
 EXPORTS = (
     "ms_custom_ops_reshape_and_cache", "ms_custom_ops_reshape_and_cache_quant",
@@ -45,6 +52,9 @@ EXPORTS = (
     "ms_custom_ops_paged_attention_with_lse", "ms_custom_ops_reshape_and_cache_infer",
     "ms_custom_ops_plan_cache_miss_stats", "ms_custom_ops_plan_arena_stats",
     "ms_custom_ops_reshape_and_cache_npd_infer", "ms_custom_ops_reshape_and_cache_npd",
+    "ms_custom_ops_rope_and_cache_infer", "ms_custom_ops_rope_and_cache", "ms_custom_ops_chunk_attention_infer",
+    "ms_custom_ops_chunk_attention_workspace_size", "ms_custom_ops_chunk_attention",
+    "ms_custom_ops_verify_draft_tokens_infer", "ms_custom_ops_verify_draft_tokens",
 )
 
 
@@ -104,6 +114,22 @@ def lib():
     L.ms_custom_ops_fa_update_infer.argtypes = [_TP, _TP, i64, i64, i32p, i32p, i64p]
     L.ms_custom_ops_fa_update.restype = C.c_int
     L.ms_custom_ops_fa_update.argtypes = [_TP, _TP, i64, i64, _TP, vp]
+    L.ms_custom_ops_rope_and_cache_infer.restype = C.c_int
+    L.ms_custom_ops_rope_and_cache_infer.argtypes = [_TP] * 10 + [C.c_double, C.c_int32, i64] + [_TP] * 5 + [i32p, i32p,
+                                                                                                       i64p]
+    L.ms_custom_ops_rope_and_cache.restype = C.c_int
+    L.ms_custom_ops_rope_and_cache.argtypes = [_TP] * 10 + [C.c_double, C.c_int32, i64] + [_TP] * 6 + [vp]
+    cp = C.POINTER(MsChunkAttentionArgs)
+    L.ms_custom_ops_chunk_attention_infer.restype = C.c_int
+    L.ms_custom_ops_chunk_attention_infer.argtypes = [cp, i32p, i32p, i64p]
+    L.ms_custom_ops_chunk_attention_workspace_size.restype = C.c_int
+    L.ms_custom_ops_chunk_attention_workspace_size.argtypes = [cp, C.POINTER(C.c_size_t)]
+    L.ms_custom_ops_chunk_attention.restype = C.c_int
+    L.ms_custom_ops_chunk_attention.argtypes = [cp, _TP, _TP, vp, C.c_size_t, vp]
+    L.ms_custom_ops_verify_draft_tokens_infer.restype = C.c_int
+    L.ms_custom_ops_verify_draft_tokens_infer.argtypes = [_TP] * 5 + [i32p, i32p, i64p]
+    L.ms_custom_ops_verify_draft_tokens.restype = C.c_int
+    L.ms_custom_ops_verify_draft_tokens.argtypes = [_TP] * 7 + [vp]
     L.ms_custom_ops_last_error.restype = C.c_char_p
     L.ms_custom_ops_last_error_kind.restype = C.c_int
     L.ms_custom_ops_num_ops.restype = C.c_int

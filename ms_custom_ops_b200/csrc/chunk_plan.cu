@@ -1,0 +1,126 @@
+// Chunk attention: checks, work list and launch (C ABI).
+#include <algorithm>
+#include <cmath>
+#include <exception>
+#include <vector>
+
+#include "chunk_params.h"
+#include "msco_common.cuh"
+
+namespace msco {
+namespace {
+
+int check_desc(const MscoChunkDesc &d) {
+  if (d.q_dtype != MSCO_DTYPE_F16 && d.q_dtype != MSCO_DTYPE_BF16)
+    return fail(MSCO_ERR_INVALID_ARG, "chunk_attention: query must be float16 or bfloat16");
+  if (d.kv_dtype != d.q_dtype && d.kv_dtype != MSCO_DTYPE_I8)
+    return fail(MSCO_ERR_INVALID_ARG, "chunk_attention: the caches must have the query's type or be int8");
+  if (d.num_q_heads <= 0 || d.num_kv_heads <= 0 || d.num_q_heads % d.num_kv_heads != 0)
+    return fail(MSCO_ERR_INVALID_ARG, "chunk_attention: q heads (%d) must be a positive multiple of kv heads (%d)",
+                d.num_q_heads, d.num_kv_heads);
+  if (d.head_dim <= 0 || d.head_dim > 256)
+    return fail(MSCO_ERR_INVALID_ARG, "chunk_attention: head_dim must be in (0, 256], got %d", d.head_dim);
+  if (d.block_size <= 0 || d.num_blocks <= 0 || d.max_blocks_per_seq < 0)
+    return fail(MSCO_ERR_INVALID_ARG, "chunk_attention: bad cache geometry");
+  if (d.cache_layout != 0 && d.cache_layout != 1)
+    return fail(MSCO_ERR_INVALID_ARG, "chunk_attention: cache_layout must be 0 (block_size major) or 1 (head major)");
+  if (d.window < 0) return fail(MSCO_ERR_INVALID_ARG, "chunk_attention: window must not be negative, got %d", d.window);
+  if (!std::isfinite(d.qk_scale)) return fail(MSCO_ERR_INVALID_ARG, "chunk_attention: qk_scale must be finite");
+  if (d.kernel != 0 && d.kernel != kChunkKernelGeneric)
+    return fail(MSCO_ERR_INVALID_ARG, "chunk_attention: kernel must be 0 or 1");
+  return MSCO_OK;
+}
+
+// The sequences with new tokens, those that see most first: their items are the longest and start first.
+int collect(const MscoChunkDesc &d, const int32_t *q_lens, const int32_t *ctx, int32_t batch,
+            std::vector<ChunkSeq> *out) {
+  if (batch < 0 || (batch > 0 && (q_lens == nullptr || ctx == nullptr)))
+    return fail(MSCO_ERR_INVALID_ARG, "chunk_attention: NULL lengths");
+  const int64_t cap = (int64_t)d.max_blocks_per_seq * d.block_size;
+  int64_t rows = 0;
+  out->clear();
+  for (int b = 0; b < batch; ++b) {
+    if (q_lens[b] < 0 || ctx[b] < 0)
+      return fail(MSCO_ERR_INVALID_ARG, "chunk_attention: q_seq_lens[%d] = %d and context_lens[%d] = %d must not be "
+                  "negative", b, q_lens[b], b, ctx[b]);
+    if (ctx[b] > cap)
+      return fail(MSCO_ERR_INVALID_ARG, "chunk_attention: context_lens[%d] = %d exceeds the block table (%d blocks of "
+                  "%d)", b, ctx[b], d.max_blocks_per_seq, d.block_size);
+    if (rows + q_lens[b] > 0x7fffffffLL) return fail(MSCO_ERR_INVALID_ARG, "chunk_attention: too many query tokens");
+    if (q_lens[b] > 0) out->push_back({0, (int32_t)rows, q_lens[b], ctx[b], b, 1, 0x7fffffff, 0});
+    rows += q_lens[b];
+  }
+  std::stable_sort(out->begin(), out->end(), [](const ChunkSeq &a, const ChunkSeq &b) { return a.ctx > b.ctx; });
+  return MSCO_OK;
+}
+
+int workspace_bytes_of(const MscoChunkDesc *desc, const int32_t *q_lens, const int32_t *ctx, int32_t batch, size_t *bytes) {
+  if (desc == nullptr || bytes == nullptr) return fail(MSCO_ERR_INVALID_ARG, "chunk_attention: NULL argument");
+  *bytes = 0;
+  if (int rc = check_desc(*desc)) return rc;
+  std::vector<ChunkSeq> seqs;
+  if (int rc = collect(*desc, q_lens, ctx, batch, &seqs)) return rc;
+  return MSCO_OK;
+}
+
+int launch(const MscoChunkDesc *desc, const int32_t *q_lens,
+                                    const int32_t *ctx, int32_t batch, const void *query,
+                                    const void *key_cache, const void *value_cache, const int32_t *block_tables,
+                                    const float *k_descale, const int32_t *k_offset, const float *v_descale,
+                                    const int32_t *v_offset, void *out, float *lse, void *workspace,
+                                    size_t workspace_bytes, int32_t *oob_count, void *stream) {
+  if (desc == nullptr) return fail(MSCO_ERR_INVALID_ARG, "chunk_attention: NULL argument");
+  const MscoChunkDesc &d = *desc;
+  if (int rc = check_desc(d)) return rc;
+  std::vector<ChunkSeq> seqs;
+  if (int rc = collect(d, q_lens, ctx, batch, &seqs)) return rc;
+  if (seqs.empty()) return MSCO_OK;
+  if (query == nullptr || key_cache == nullptr || value_cache == nullptr || out == nullptr ||
+      (block_tables == nullptr && d.max_blocks_per_seq > 0))
+    return fail(MSCO_ERR_INVALID_ARG, "chunk_attention: query, caches, block_tables and out must not be NULL");
+  if (d.kv_dtype == MSCO_DTYPE_I8 && (k_descale == nullptr || v_descale == nullptr))
+    return fail(MSCO_ERR_INVALID_ARG, "chunk_attention: int8 caches need k_descale and v_descale");
+  (void)workspace;
+  (void)workspace_bytes;
+  ChunkParams p = {};
+  p.q = query; p.key_cache = key_cache; p.value_cache = value_cache; p.block_tables = block_tables;
+  p.k_descale = k_descale; p.k_offset = k_offset; p.v_descale = v_descale; p.v_offset = v_offset;
+  p.out = out; p.lse = lse; p.oob_count = oob_count;
+  p.num_blocks = d.num_blocks;
+  p.num_q_heads = d.num_q_heads; p.num_kv_heads = d.num_kv_heads; p.head_dim = d.head_dim;
+  p.block_size = d.block_size; p.max_blocks_per_seq = d.max_blocks_per_seq; p.cache_layout = d.cache_layout;
+  p.group = d.num_q_heads / d.num_kv_heads;
+  p.window = d.window;
+  p.scale_log2e = (float)((double)d.qk_scale * 1.4426950408889634);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  for (size_t at = 0; at < seqs.size(); at += kChunkSeqsMax) {
+    p.nseq = (int)std::min<size_t>(kChunkSeqsMax, seqs.size() - at);
+    if (int rc = launch_chunk_generic(d, p, seqs.data() + at, st)) return rc;
+  }
+  return MSCO_OK;
+}
+
+}  // namespace
+}  // namespace msco
+
+using namespace msco;
+
+// Exceptions of the host containers end here: the callers are C.
+extern "C" int msco_chunk_attention_workspace(const MscoChunkDesc *desc, const int32_t *host_q_seq_lens,
+                                              const int32_t *host_context_lens, int32_t batch, size_t *bytes) try {
+  return workspace_bytes_of(desc, host_q_seq_lens, host_context_lens, batch, bytes);
+} catch (const std::exception &e) {
+  return fail(MSCO_ERR_INTERNAL, "chunk_attention: %s", e.what());
+}
+
+extern "C" int msco_chunk_attention(const MscoChunkDesc *desc, const int32_t *host_q_seq_lens,
+                                    const int32_t *host_context_lens, int32_t batch, const void *query,
+                                    const void *key_cache, const void *value_cache, const int32_t *block_tables,
+                                    const float *k_descale, const int32_t *k_offset, const float *v_descale,
+                                    const int32_t *v_offset, void *out, float *lse, void *workspace,
+                                    size_t workspace_bytes, int32_t *oob_count, void *stream) try {
+  return launch(desc, host_q_seq_lens, host_context_lens, batch, query, key_cache, value_cache, block_tables, k_descale,
+                k_offset, v_descale, v_offset, out, lse, workspace, workspace_bytes, oob_count, stream);
+} catch (const std::exception &e) {
+  return fail(MSCO_ERR_INTERNAL, "chunk_attention: %s", e.what());
+}

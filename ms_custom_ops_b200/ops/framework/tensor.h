@@ -101,9 +101,9 @@ class Tensor {
       if (d_->shape[i] == 0) return true;
     return false;
   }
-  // Row-major contiguity (dimensions of extent 1 may carry any stride).
+  // Row-major contiguity (dimensions of extent 1, and empty tensors, may carry any stride).
   bool is_contiguous() const {
-    if (!d_) return true;
+    if (!d_ || has_zero_dim()) return true;
     int64_t expect = 1;
     for (int i = d_->ndim - 1; i >= 0; --i) {
       if (d_->shape[i] != 1 && d_->strides[i] != expect) return false;
