@@ -492,6 +492,10 @@ int msco_chunk_attention(const MscoChunkDesc *desc, const int32_t *host_q_seq_le
                          const int32_t *v_offset, void *out, float *lse, void *workspace,
                          size_t workspace_bytes, int32_t *oob_count, void *stream);
 
+/* MSCO_ERR_TIMEOUT once a bounded wait of a chunk_attention kernel has run out on the current device since the
+ * process started, else MSCO_OK.  Synchronises (a copy of one word). */
+int msco_chunk_attention_status(void);
+
 /* ------------------------------------------------------------------------
  * verify_draft_tokens (extension): rejection sampling of drafted tokens against the target's probabilities.
  *   target_probs [batch, drafts + 1, vocab], draft_probs [batch, drafts, vocab] (F32 / F16 / BF16, the same type) or

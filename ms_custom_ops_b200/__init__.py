@@ -36,7 +36,8 @@ __all__ = ["reshape_and_cache", "reshape_and_cache_infer", "reshape_and_cache_np
            "paged_attention_infer", "plan_arena_stats",
            "paged_cache_load", "paged_cache_load_infer", "fa_update", "fa_update_infer", "paged_attention_with_lse",
            "paged_attention_workspace_size", "paged_attention_check_status", "rope_and_cache", "rope_and_cache_infer",
-           "chunk_attention", "chunk_attention_infer", "chunk_attention_workspace_size", "verify_draft_tokens",
+           "chunk_attention", "chunk_attention_infer", "chunk_attention_workspace_size",
+           "chunk_attention_check_status", "verify_draft_tokens",
            "verify_draft_tokens_infer", "TensorSpec", "MscoError",
            "UnsupportedOnB200", "registered_ops", "plan_cache_stats", "plan_cache_clear"]
 
@@ -713,6 +714,16 @@ def chunk_attention_workspace_size(query, key_cache, value_cache, block_tables, 
     n = C.c_size_t()
     _host.check(_host.lib().ms_custom_ops_chunk_attention_workspace_size(C.byref(a), C.byref(n)))
     return int(n.value)
+
+
+def chunk_attention_check_status(device=None):
+    """Synchronise the current stream of `device` and raise if a bounded wait of a chunk_attention kernel has run out on
+    it (MSCO_ERR_TIMEOUT) since the process started."""
+    import torch
+    device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    with torch.cuda.device(device):
+        torch.cuda.current_stream(device).synchronize()
+        _abi.check(_abi.lib().msco_chunk_attention_status())
 
 
 def verify_draft_tokens(target_probs, draft_probs, draft_tokens, uniform, draft_lens=None):

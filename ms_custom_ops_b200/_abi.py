@@ -80,7 +80,8 @@ EXPORTS = (
     "msco_paged_attention_launch_lse", "msco_expand_rows_i32", "msco_paged_attention_replan", "msco_plan_arena_stats",
     "msco_reshape_and_cache_bnsd", "msco_copy_device", "msco_paged_attention_plan_tokens",
     "msco_paged_attention_replan_tokens", "msco_paged_attention_tma_supported", "msco_paged_cache_load_workspace_bytes", "msco_paged_cache_load", "msco_fa_update", "msco_fa_update_strided",
-    "msco_rope_and_cache", "msco_chunk_attention_workspace", "msco_chunk_attention", "msco_verify_draft_tokens",
+    "msco_rope_and_cache", "msco_chunk_attention_workspace", "msco_chunk_attention",
+    "msco_chunk_attention_status", "msco_verify_draft_tokens",
 )
 
 
@@ -119,6 +120,8 @@ def lib():
     L.msco_chunk_attention_workspace.argtypes = [C.POINTER(MscoChunkDesc), vp, vp, i32, C.POINTER(sz)]
     L.msco_chunk_attention.restype = C.c_int
     L.msco_chunk_attention.argtypes = [C.POINTER(MscoChunkDesc), vp, vp, i32] + [vp] * 11 + [sz, vp, vp]
+    L.msco_chunk_attention_status.restype = C.c_int
+    L.msco_chunk_attention_status.argtypes = []
     L.msco_verify_draft_tokens.restype = C.c_int
     L.msco_verify_draft_tokens.argtypes = [vp, vp, i32] + [vp] * 5 + [i32] * 3 + [vp]
     L.msco_paged_attention_split_tokens.restype = i32

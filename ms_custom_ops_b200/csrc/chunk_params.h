@@ -22,7 +22,7 @@ struct ChunkSeq {
   int32_t row;        // block-table row
   int32_t nsplit;     // KV splits of every query tile
   int32_t chunk;      // KV tiles per split
-  int32_t part_base;  // first partial tile (nsplit > 1): (query tile * nsplit + split) * kv_heads + kv head follows
+  int32_t part_base;  // first partial row (nsplit > 1); its tiles are numbered (query tile * nsplit + split) * kv_heads + kv head
 };
 
 struct ChunkParams {
@@ -36,14 +36,13 @@ struct ChunkParams {
   const int32_t *v_offset;
   void *out;
   float *lse;          // optional [tokens, num_q_heads], natural logarithm
-  float *part_o;       // [partial tile, rows_per_item, head_dim] un-normalised partial outputs
-  float *part_ml;      // [partial tile, rows_per_item, 2] running max (log2 domain) and sum
+  float *part_o;       // [partial row, head_dim] un-normalised partial outputs
+  float *part_ml;      // [partial row, 2] running max (log2 domain) and sum
   int32_t *oob_count;  // optional: block ids outside the cache
   int64_t num_blocks;
   int num_q_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq, cache_layout;
   int group;           // q heads per kv head
-  int item_tokens;     // new tokens of one item
-  int rows_per_item;   // rows of a partial tile
+  int item_tokens;     // new tokens of one item (two streams of item_tokens / 2)
   int window;          // 0: none
   float scale_log2e;   // qk_scale * log2(e)
   int nseq, items;
@@ -98,6 +97,9 @@ __device__ __forceinline__ ChunkItem chunk_item(const ChunkSeqs<N> &seqs, const 
 
 // launchers (defined next to the kernels)
 bool chunk_tc_supported(const MscoChunkDesc &d);
+int launch_chunk_tc(const MscoChunkDesc &d, const ChunkParams &p, const ChunkSeq *seqs, int64_t q_rows, int sms,
+                    cudaStream_t stream);
+int chunk_tc_status();  // MSCO_OK, or MSCO_ERR_TIMEOUT once a bounded wait ran out on the current device (synchronises)
 int launch_chunk_generic(const MscoChunkDesc &d, const ChunkParams &p, const ChunkSeq *seqs, cudaStream_t stream);
 
 }  // namespace msco

@@ -54,34 +54,101 @@ int collect(const MscoChunkDesc &d, const int32_t *q_lens, const int32_t *ctx, i
   return MSCO_OK;
 }
 
+bool use_tc(const MscoChunkDesc &d) { return d.kernel != kChunkKernelGeneric && chunk_tc_supported(d); }
+int item_tokens_of(const MscoChunkDesc &d) { return 2 * (kChunkKvTile / (d.num_q_heads / d.num_kv_heads)); }
+
+// KV splits of the tensor-core kernel.  A function of the sequence's own lengths and of the head counts, so that the
+// result of a sequence does not depend on the others of the call.
+void split_rule(const MscoChunkDesc &d, ChunkSeq *e) {
+  const int group = d.num_q_heads / d.num_kv_heads, it = item_tokens_of(d);
+  const int64_t alone = (int64_t)((e->q_len + it - 1) / it) * d.num_kv_heads;  // items without splits
+  // KV tiles of the longest item
+  const int last0 = (e->q_len - 1) / it * it;
+  const int hi = e->ctx, lo = d.window > 0 ? std::max(0, e->ctx - e->q_len + last0 - d.window + 1) : 0;
+  const int tiles = hi > lo ? (hi + kChunkKvTile - 1) / kChunkKvTile - lo / kChunkKvTile : 0;
+  const int rows = std::min(e->q_len, it) * group;
+  const int min_tiles = rows <= 32 ? 4 : (rows <= 128 ? 8 : 24);
+  const int64_t want = std::max<int64_t>(1, 296 / alone);
+  const int nsplit = (int)std::max<int64_t>(1, std::min<int64_t>(want, tiles / min_tiles));
+  e->chunk = nsplit > 1 ? (tiles + nsplit - 1) / nsplit : 0x3fffffff;
+  e->nsplit = nsplit > 1 ? (tiles + e->chunk - 1) / e->chunk : 1;
+  // windows: an earlier item may touch one tile more than the last one
+  if (e->nsplit > 1 && d.window > 0) e->nsplit += 1;
+}
+
+struct Plan {
+  std::vector<ChunkSeq> seqs;
+  std::vector<int64_t> items;  // of every launch (group of kChunkSeqsMax sequences)
+  int64_t part_rows = 0, q_rows = 0;
+};
+
+int make_plan(const MscoChunkDesc &d, const int32_t *q_lens, const int32_t *ctx, int32_t batch, Plan *pl) {
+  if (int rc = collect(d, q_lens, ctx, batch, &pl->seqs)) return rc;
+  for (const ChunkSeq &e : pl->seqs) pl->q_rows += e.q_len;
+  if (!use_tc(d)) return MSCO_OK;
+  const int it = item_tokens_of(d), group = d.num_q_heads / d.num_kv_heads;
+  for (size_t i = 0; i < pl->seqs.size(); ++i) {
+    if (i % kChunkSeqsMax == 0) pl->items.push_back(0);
+    ChunkSeq &e = pl->seqs[i];
+    split_rule(d, &e);
+    const int64_t tiles = ((int64_t)e.q_len + it - 1) / it * e.nsplit * d.num_kv_heads;
+    e.item_base = (int32_t)pl->items.back();
+    pl->items.back() += tiles;
+    if (e.nsplit > 1) {
+      e.part_base = (int32_t)pl->part_rows;
+      pl->part_rows += tiles * std::min(e.q_len, it) * group;
+    }
+    if (pl->items.back() > 0x3fffffffLL || pl->part_rows > 0x7fffffffLL)
+      return fail(MSCO_ERR_INVALID_ARG, "chunk_attention: too many work items");
+  }
+  return MSCO_OK;
+}
+
+size_t part_ml_offset(const MscoChunkDesc &d, const Plan &pl) {
+  return ((size_t)pl.part_rows * d.head_dim * 4 + 255) / 256 * 256;
+}
+size_t bytes_of(const MscoChunkDesc &d, const Plan &pl) {
+  return pl.part_rows == 0 ? 0 : part_ml_offset(d, pl) + (size_t)pl.part_rows * 8;
+}
+
 int workspace_bytes_of(const MscoChunkDesc *desc, const int32_t *q_lens, const int32_t *ctx, int32_t batch, size_t *bytes) {
   if (desc == nullptr || bytes == nullptr) return fail(MSCO_ERR_INVALID_ARG, "chunk_attention: NULL argument");
   *bytes = 0;
   if (int rc = check_desc(*desc)) return rc;
-  std::vector<ChunkSeq> seqs;
-  if (int rc = collect(*desc, q_lens, ctx, batch, &seqs)) return rc;
+  Plan pl;
+  if (int rc = make_plan(*desc, q_lens, ctx, batch, &pl)) return rc;
+  *bytes = bytes_of(*desc, pl);
   return MSCO_OK;
 }
 
-int launch(const MscoChunkDesc *desc, const int32_t *q_lens,
-                                    const int32_t *ctx, int32_t batch, const void *query,
-                                    const void *key_cache, const void *value_cache, const int32_t *block_tables,
-                                    const float *k_descale, const int32_t *k_offset, const float *v_descale,
-                                    const int32_t *v_offset, void *out, float *lse, void *workspace,
-                                    size_t workspace_bytes, int32_t *oob_count, void *stream) {
+int sm_count() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) == cudaSuccess && cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess &&
+      n > 0)
+    return n;
+  (void)cudaGetLastError();
+  return 148;
+}
+
+int launch(const MscoChunkDesc *desc, const int32_t *q_lens, const int32_t *ctx, int32_t batch, const void *query,
+           const void *key_cache, const void *value_cache, const int32_t *block_tables, const float *k_descale,
+           const int32_t *k_offset, const float *v_descale, const int32_t *v_offset, void *out, float *lse,
+           void *workspace, size_t workspace_bytes, int32_t *oob_count, void *stream) {
   if (desc == nullptr) return fail(MSCO_ERR_INVALID_ARG, "chunk_attention: NULL argument");
   const MscoChunkDesc &d = *desc;
   if (int rc = check_desc(d)) return rc;
-  std::vector<ChunkSeq> seqs;
-  if (int rc = collect(d, q_lens, ctx, batch, &seqs)) return rc;
-  if (seqs.empty()) return MSCO_OK;
+  Plan pl;
+  if (int rc = make_plan(d, q_lens, ctx, batch, &pl)) return rc;
+  if (pl.seqs.empty()) return MSCO_OK;
   if (query == nullptr || key_cache == nullptr || value_cache == nullptr || out == nullptr ||
       (block_tables == nullptr && d.max_blocks_per_seq > 0))
     return fail(MSCO_ERR_INVALID_ARG, "chunk_attention: query, caches, block_tables and out must not be NULL");
   if (d.kv_dtype == MSCO_DTYPE_I8 && (k_descale == nullptr || v_descale == nullptr))
     return fail(MSCO_ERR_INVALID_ARG, "chunk_attention: int8 caches need k_descale and v_descale");
-  (void)workspace;
-  (void)workspace_bytes;
+  const size_t need = bytes_of(d, pl);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0))
+    return fail(MSCO_ERR_INVALID_ARG, "chunk_attention: the workspace must be 256-byte aligned and hold %zu bytes, got %zu",
+                need, workspace_bytes);
   ChunkParams p = {};
   p.q = query; p.key_cache = key_cache; p.value_cache = value_cache; p.block_tables = block_tables;
   p.k_descale = k_descale; p.k_offset = k_offset; p.v_descale = v_descale; p.v_offset = v_offset;
@@ -92,10 +159,23 @@ int launch(const MscoChunkDesc *desc, const int32_t *q_lens,
   p.group = d.num_q_heads / d.num_kv_heads;
   p.window = d.window;
   p.scale_log2e = (float)((double)d.qk_scale * 1.4426950408889634);
+  bool tc = use_tc(d);
+  if (tc) {
+    p.item_tokens = item_tokens_of(d);
+    p.part_o = static_cast<float *>(workspace);
+    p.part_ml = reinterpret_cast<float *>(static_cast<char *>(workspace) + part_ml_offset(d, pl));
+    if (((reinterpret_cast<uintptr_t>(query) | reinterpret_cast<uintptr_t>(key_cache) |
+          reinterpret_cast<uintptr_t>(value_cache) | reinterpret_cast<uintptr_t>(out)) & 15) != 0)
+      tc = false;  // rows that the copies cannot start on: the general kernel takes them
+  }
+  const int sms = tc ? sm_count() : 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  for (size_t at = 0; at < seqs.size(); at += kChunkSeqsMax) {
-    p.nseq = (int)std::min<size_t>(kChunkSeqsMax, seqs.size() - at);
-    if (int rc = launch_chunk_generic(d, p, seqs.data() + at, st)) return rc;
+  for (size_t at = 0; at < pl.seqs.size(); at += kChunkSeqsMax) {
+    p.nseq = (int)std::min<size_t>(kChunkSeqsMax, pl.seqs.size() - at);
+    if (tc) p.items = (int)pl.items[at / kChunkSeqsMax];
+    if (int rc = tc ? launch_chunk_tc(d, p, pl.seqs.data() + at, pl.q_rows, sms, st)
+                    : launch_chunk_generic(d, p, pl.seqs.data() + at, st))
+      return rc;
   }
   return MSCO_OK;
 }
@@ -123,4 +203,12 @@ extern "C" int msco_chunk_attention(const MscoChunkDesc *desc, const int32_t *ho
                 k_offset, v_descale, v_offset, out, lse, workspace, workspace_bytes, oob_count, stream);
 } catch (const std::exception &e) {
   return fail(MSCO_ERR_INTERNAL, "chunk_attention: %s", e.what());
+}
+
+extern "C" int msco_chunk_attention_status(void) {
+  const int rc = chunk_tc_status();
+  if (rc == MSCO_ERR_TIMEOUT)
+    return fail(rc, "chunk_attention: a bounded device-side wait ran out on this device; results of that launch are not valid");
+  if (rc != MSCO_OK) return fail(rc, "chunk_attention: the error word of the device cannot be read");
+  return MSCO_OK;
 }

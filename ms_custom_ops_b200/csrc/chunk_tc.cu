@@ -1,0 +1,690 @@
+// Chunk attention on the 5th-generation tensor cores: head_dim 64 / 128, 16-bit caches.
+//
+// An item is up to 256 packed rows of one kv head (token-major, the q heads of the group adjacent) against the
+// cached tokens that they see, or a split of them, 128 at a time.  Two streams keep the tensor cores busy:
+// while one stream's 128 rows are in their softmax, the other's products run.
+//   rows > 128   ("dual")   stream s owns rows 128 s .. 128 s + 127, both go over all KV tiles
+//   rows <= 128  ("single") both streams own the same rows, stream s the KV tiles s, s + 2, ...; their states
+//                           are merged at the end
+// Per tile and stream:  S = Q K^T (shared x shared -> TMEM),  P = 2^(S scale - m) (registers, one row per thread, back
+// to TMEM in 16 bits over S),  O += P V (TMEM x shared -> TMEM).  The running maximum only moves when it grows by
+// more than kSlack (a factor 256): until then P is up to 256 instead of 1, which costs no precision in a floating
+// format, and O stays where it is; it is rescaled in TMEM by the softmax warps in the rare tiles where it must.
+//
+// Warps: 0-3 / 4-7 softmax of stream 0 / 1, 8 loads (TMA, 128-byte swizzle), 9 matrix instructions (10, 11 idle: registers
+// are handed out by groups of four warps).
+// The matrix instructions are issued O_0 += P_0 V, S_0 = Q_0 K', O_1 += P_1 V, S_1 = Q_1 K' (K' the next tile); they execute in
+// that order, so a completed S' means that the product that read P, which lies over it, is complete too.
+#include <cuda.h>
+
+#include <algorithm>
+#include <mutex>
+
+#include "chunk_params.h"
+#include "msco_common.cuh"
+#include "tc05.cuh"
+
+namespace msco {
+namespace {
+
+constexpr int kRows = 128;        // rows of one stream
+constexpr int kTile = kChunkKvTile;
+constexpr int kThreads = 384;
+constexpr float kSlack = 8.f;     // log2 of how far a probability may exceed 1
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr uint32_t kWaitLimit = 1u << 22;
+
+__device__ int g_chunk_error;  // MSCO_ERR_TIMEOUT once a bounded wait has run out
+
+template <int D>
+struct Cfg {
+  static_assert(D == 64 || D == 128, "head_dim 64 or 128");
+  static constexpr int kBoxes = D / 64;                 // 128-byte wide sub-tiles of a row
+  static constexpr int kSub = kTile * 128;              // bytes of one sub-tile
+  static constexpr int kStageBytes = kTile * D * 2;
+  static constexpr int kQBytes = kRows * D * 2;
+  static constexpr int kStages = D == 128 ? 5 : 10;
+  static constexpr int kOffKv = 2 * kQBytes;
+  static constexpr int kOffBar = kOffKv + kStages * kStageBytes;
+  static constexpr int kNumBars = 2 * kStages + 10;
+  static constexpr int kOffMl = kOffBar + kNumBars * 8 + 16;  // [128][2] floats of the merge of the streams
+  static constexpr int kSmem = kOffMl + kRows * 2 * 4;
+  static constexpr int kDynSmem = kSmem + 1024;
+  static constexpr int kColO = 2 * kTile;               // TMEM columns: S_0, S_1, O_0, O_1
+};
+
+// A bounded wait on an mbarrier.  Should one run out (a lost arrival), the block's flag is set, every wait of the block
+// returns at once from then on, and all roles run through the rest of their loops without waiting: whatever they do
+// stays inside their buffers, the result is worthless and the device's error word says so.
+struct Waiter {
+  volatile int *abort;
+  __device__ __forceinline__ void operator()(uint64_t *bar, uint32_t parity) const {
+    for (uint32_t i = 0; i < kWaitLimit; ++i) {
+      if (mbar_try_wait(bar, parity)) return;
+      if (*abort) return;
+    }
+    *abort = 1;
+    atomicExch(&g_chunk_error, MSCO_ERR_TIMEOUT);
+  }
+};
+
+// Everything about an item that the roles share.
+struct Work {
+  ChunkItem it;
+  int n;        // KV tiles
+  int dual;
+  int t1;       // first token of stream 1's rows (dual)
+  int j0[2], j1[2];  // tiles of each stream, absolute
+  int step;     // 1 (dual) or 2
+};
+
+template <int N>
+__device__ __forceinline__ Work make_work(const ChunkSeqs<N> &seqs, const ChunkParams &p, int item) {
+  Work w;
+  w.it = chunk_item(seqs, p, item);
+  const ChunkSeq &e = seqs.s[w.it.seq];
+  const int half = p.item_tokens >> 1;
+  w.n = max(0, w.it.tile1 - w.it.tile0);
+  w.dual = w.it.tok1 - w.it.tok0 > half;
+  w.t1 = w.it.tok0 + half;
+  w.step = w.dual ? 1 : 2;
+  if (w.dual) {
+    // tiles that no row of the stream sees are left out: behind the last token of stream 0's rows, in front of
+    // the window of stream 1's first
+    const int pos0 = e.ctx - e.q_len;
+    const int end0 = (max(0, pos0 + w.t1) + kTile - 1) / kTile;
+    const int beg1 = p.window > 0 ? max(0, pos0 + w.t1 - p.window + 1) / kTile : 0;
+    w.j0[0] = w.it.tile0;
+    w.j1[0] = max(w.it.tile0, min(w.it.tile1, end0));
+    w.j0[1] = min(max(w.it.tile0, beg1), max(w.it.tile0, w.it.tile1));
+    w.j1[1] = max(w.it.tile0, w.it.tile1);
+  } else {
+    w.j0[0] = w.it.tile0;
+    w.j0[1] = w.it.tile0 + 1;
+    w.j1[0] = w.j1[1] = max(w.it.tile0, w.it.tile1);
+  }
+  return w;
+}
+
+// item of round `r` of this CTA: rounds go forth and back over the CTAs (the list is longest first)
+__device__ __forceinline__ int item_of(int r) {
+  const int g = (int)gridDim.x, c = (int)blockIdx.x;
+  return r * g + ((r & 1) ? g - 1 - c : c);
+}
+
+template <typename T, int D, int N>
+__global__ void __launch_bounds__(kThreads, 1)
+chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ ChunkParams p,
+                const __grid_constant__ ChunkSeqs<N> seqs) {
+  using C = Cfg<D>;
+  constexpr bool kBf16 = sizeof(T) == 2 && !std::is_same<T, __half>::value;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t *bars = reinterpret_cast<uint64_t *>(smem + C::kOffBar);
+  uint64_t *kv_full = bars, *kv_empty = bars + C::kStages;
+  uint64_t *q_full = bars + 2 * C::kStages, *q_empty = q_full + 1, *s_full = q_full + 2, *p_full = q_full + 4,
+           *o_full = q_full + 6, *tail = q_full + 8, *fin = q_full + 9;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + C::kNumBars);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+  float *ml = reinterpret_cast<float *>(smem + C::kOffMl);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < C::kStages; ++i) {
+      mbar_init(&kv_full[i], 1);
+      mbar_init(&kv_empty[i], 1);
+    }
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 2);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&s_full[s], 1);
+      mbar_init(&p_full[s], 4);
+      mbar_init(&o_full[s], 1);
+    }
+    mbar_init(tail, 1);
+    mbar_init(fin, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 9) tmem_alloc(tmem_slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const Waiter wait{abort_flag};
+  const int half = p.item_tokens >> 1;
+
+  // Registers: 384 x 168 at launch = 256 x 208 (softmax) + 128 x 88 (the other four warps, two of them idle)
+  if (warp >= 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+  if (warp == 8) {
+    // ------------------------------------------------------------------ loads
+    if (lane == 0) {
+      prefetch_tmap(&tm_q);
+      prefetch_tmap(&tm_k);
+      prefetch_tmap(&tm_v);
+    }
+    const int bs = p.block_size;
+    const int box_rows = min(bs, kTile), boxes = kTile / box_rows;
+    uint32_t c = 0, q_round = 0, tails = 0;  // ring position, items so far, waits on `tail` so far
+    for (int r = 0, item = item_of(0); item < p.items; item = item_of(++r)) {
+      const Work w = make_work(seqs, p, item);
+      if (w.n == 0) continue;
+      const ChunkSeq &e = seqs.s[w.it.seq];
+      // cached tokens that some new token of the sequence sees: the rest of the table may hold anything
+      const int alive0 = p.window > 0 ? max(0, e.ctx - e.q_len - p.window + 1) : 0, alive1 = e.ctx;
+      const int32_t *table = p.block_tables + (int64_t)e.row * p.max_blocks_per_seq;
+      if (q_round > 0) wait(q_empty, (q_round - 1) & 1);
+      ++q_round;
+      if (lane == 0) {
+        const int tiles = w.dual ? 2 : 1;
+        mbar_arrive_expect_tx(q_full, (uint32_t)(tiles * C::kBoxes * half * p.group * 128));
+        for (int s = 0; s < tiles; ++s)
+          for (int x = 0; x < C::kBoxes; ++x)
+            tma_load_3d(smem + s * C::kQBytes + x * (kRows * 128), &tm_q, x * 64, w.it.kvh * p.group,
+                        e.q_start + (s == 0 ? w.it.tok0 : w.t1), q_full);
+      }
+      int win = -1;        // first block-table column of the 32 ids that the lanes hold
+      int32_t id = 0;
+      // one tile of K or V into the next stage of the ring
+      auto load = [&](const CUtensorMap *tm, int j, bool is_v) {
+        const uint32_t st = c % C::kStages, use = c / C::kStages;
+        ++c;
+        if (use > 0) wait(&kv_empty[st], (use - 1) & 1);
+        __syncwarp();
+        uint8_t *dst = smem + C::kOffKv + st * C::kStageBytes;
+        const int tok = j * kTile;
+        const int a = max(0, alive0 - tok), b = min(kTile, alive1 - tok);  // rows of the tile that are alive
+        const int b0 = a / box_rows, b1 = (b + box_rows - 1) / box_rows;   // boxes that hold some of them
+        // a V row that is not alive is zeroed: its probability is 0, but what it holds may not be finite
+        const bool patch = is_v && (a > 0 || b < kTile);
+        uint64_t *bar = patch ? tail : &kv_full[st];
+        const int col = (tok + lane * box_rows) / bs;  // this lane's block-table column (boxes <= 16)
+        const int first = tok / bs;
+        if (win < 0 || first < win || (tok + kTile - 1) / bs >= win + 32) {
+          win = first;
+          const int wc = win + lane;
+          id = wc < p.max_blocks_per_seq && (int64_t)wc * bs < alive1 ? __ldg(table + wc) : 0;
+        }
+        const bool mine = lane >= b0 && lane < b1 && lane < boxes;
+        int32_t blk = __shfl_sync(0xffffffffu, id, mine ? col - win : 0);
+        if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)((b1 - b0) * box_rows * 128 * C::kBoxes));
+        __syncwarp();
+        if (mine) {
+          if (blk < 0 || blk >= p.num_blocks) {
+            if (p.oob_count != nullptr && !is_v) atomicAdd(p.oob_count, 1);
+            blk = 0;
+          }
+          const int off = (tok + lane * box_rows) % bs;
+          const int y = p.cache_layout == 1 ? off : w.it.kvh;
+          const int z = p.cache_layout == 1 ? blk * p.num_kv_heads + w.it.kvh : blk * bs + off;
+#pragma unroll
+          for (int x = 0; x < C::kBoxes; ++x) tma_load_3d(dst + x * C::kSub + lane * box_rows * 128, tm, x * 64, y, z, bar);
+        }
+        if (patch) {
+          wait(tail, tails & 1);
+          ++tails;
+          __syncwarp();
+          for (int i = lane; i < kTile * 8 * C::kBoxes; i += 32) {  // 16-byte pieces; a row is 128 bytes of a sub-tile
+            const int x = i / (kTile * 8), row = (i / 8) % kTile;
+            if (row < a || row >= b)
+              *reinterpret_cast<uint4 *>(dst + x * C::kSub + row * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&kv_full[st]);
+        }
+      };
+      // the order in which the tiles are used: V of a tile right in front of the K that follows it on its stream
+      const int ahead = w.step;
+      for (int i = 0; i < min(ahead, w.n); ++i) load(&tm_k, w.it.tile0 + i, false);
+      for (int i = 0; i < w.n; ++i) {
+        load(&tm_v, w.it.tile0 + i, true);
+        if (i + ahead < w.n) load(&tm_k, w.it.tile0 + i + ahead, false);
+      }
+    }
+  } else if (warp == 9) {
+    // ------------------------------------------------------------------ matrix instructions
+    if (lane == 0) {
+      constexpr uint32_t kIdQk = mma_idesc<kBf16, kRows, kTile, false>();
+      constexpr uint32_t kIdPv = mma_idesc<kBf16, kRows, D, true>();
+      const uint32_t q_addr = smem_u32(smem), kv_addr = smem_u32(smem + C::kOffKv);
+      uint32_t c = 0, q_round = 0, p_round[2] = {0, 0};
+      for (int r = 0, item = item_of(0); item < p.items; item = item_of(++r)) {
+        const Work w = make_work(seqs, p, item);
+        if (w.n == 0) continue;
+        wait(q_full, q_round & 1);
+        ++q_round;
+        auto qk = [&](int s, uint32_t st) {
+          uint64_t a = smem_desc(q_addr + (w.dual ? s * C::kQBytes : 0)), b = smem_desc(kv_addr + st * C::kStageBytes);
+          asm volatile("" : "+l"(a), "+l"(b));  // the eight descriptors are one addition each, not values to keep
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) {
+            const uint32_t off = ((k / 4) * (kRows * 128) + (k % 4) * 32) >> 4;
+            mma_ss(tmem + s * kTile, a + off, b + off, kIdQk, k > 0);
+          }
+          tc_commit(&s_full[s]);
+        };
+        auto pv = [&](int s, uint32_t st, bool acc) {
+          wait(&p_full[s], p_round[s] & 1);
+          ++p_round[s];
+          tc_fence_after();
+          uint64_t b = smem_desc(kv_addr + st * C::kStageBytes, C::kSub);
+          asm volatile("" : "+l"(b));
+#pragma unroll
+          for (int k = 0; k < kTile / 16; ++k)
+            mma_ts(tmem + C::kColO + s * D, tmem + s * kTile + k * 8, b + (k * 2048 >> 4), kIdPv, acc || k > 0);
+        };
+        auto take = [&]() {  // the next stage of the ring, filled
+          const uint32_t st = c % C::kStages;
+          wait(&kv_full[st], (c / C::kStages) & 1);
+          ++c;
+          tc_fence_after();
+          return st;
+        };
+        if (w.dual) {
+          for (int j = w.it.tile0 - 1; j < w.it.tile1; ++j) {
+            // V of tile j, then K of tile j + 1; the streams alternate
+            const bool has_v = j >= w.it.tile0, has_k = j + 1 < w.it.tile1;
+            const uint32_t sv = has_v ? take() : 0, sk = has_k ? take() : 0;
+#pragma unroll 1
+            for (int s = 0; s < 2; ++s) {
+              if (has_v && j >= w.j0[s] && j < w.j1[s]) {
+                pv(s, sv, j > w.j0[s]);
+                if (j + 1 == w.j1[s]) tc_commit(&o_full[s]);
+              }
+              if (s == 1 && has_v) tc_commit(&kv_empty[sv]);
+              if (has_k && j + 1 >= w.j0[s] && j + 1 < w.j1[s]) qk(s, sk);
+            }
+            if (has_k) {
+              tc_commit(&kv_empty[sk]);
+              if (j + 2 >= w.it.tile1) tc_commit(q_empty);
+            }
+          }
+        } else {
+          for (int i = 0; i < min(2, w.n); ++i) {
+            const uint32_t st = take();
+            qk(i, st);
+            tc_commit(&kv_empty[st]);
+            if (i + 1 == w.n) tc_commit(q_empty);
+          }
+          for (int i = 0; i < w.n; ++i) {
+            const int s = i & 1;
+            const uint32_t sv = take();
+            pv(s, sv, i > 1);
+            tc_commit(&kv_empty[sv]);
+            if (i + 2 >= w.n) {
+              tc_commit(&o_full[s]);
+              continue;
+            }
+            const uint32_t sk = take();
+            qk(s, sk);
+            tc_commit(&kv_empty[sk]);
+            if (i + 3 == w.n) tc_commit(q_empty);
+          }
+        }
+      }
+      tc_commit(fin);  // every arrival that the instructions still owe has happened before the block ends
+      wait(fin, 0);
+    }
+    __syncwarp();
+  } else if (warp < 8) {
+    // ------------------------------------------------------------------ softmax, one row per thread
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    const int s = warp >> 2;
+    const int row = threadIdx.x & 127;
+    const uint32_t lanes = (uint32_t)(warp & 3) * 32 << 16;
+    const uint32_t t_s = tmem + lanes + s * kTile, t_o = tmem + lanes + C::kColO + s * D;
+    const int g = p.group;
+    const int tok_in = row / g, head_in = row - tok_in * g;
+    uint32_t s_round = 0, o_round = 0, q_round = 0;
+    for (int r = 0, item = item_of(0); item < p.items; item = item_of(++r)) {
+      const Work w = make_work(seqs, p, item);
+      const ChunkSeq &e = seqs.s[w.it.seq];
+      const int tok0 = w.dual && s == 1 ? w.t1 : w.it.tok0;
+      const int ntok = min(half, w.it.tok1 - tok0);
+      const bool live = tok_in < ntok;  // this thread has a row
+      const bool warp_live = __any_sync(0xffffffffu, live);
+      const int pos0 = e.ctx - e.q_len + tok0;
+      const int pos = live ? pos0 + tok_in : -1;
+      float m = -INFINITY, l = 0.f;
+      if (warp == 4 && w.n > 0) {
+        // One of the two arrivals that free Q's space is stream 1's: at once (dual), or when the merge is through with it
+        // (single).  It comes behind the arrival of the item's rows, so never before the one of the item in front.
+        wait(q_full, q_round & 1);
+        ++q_round;
+        if (w.dual && lane == 0) mbar_arrive(q_empty);
+      }
+      for (int j = w.j0[s]; j < w.j1[s]; j += w.step) {
+        wait(&s_full[s], s_round & 1);
+        ++s_round;
+        __syncwarp();
+        tc_fence_after();
+        if (warp_live) {
+          uint32_t x[kTile];
+#pragma unroll
+          for (int c = 0; c < kTile; c += 32) tmem_ld32(t_s + c, x + c);
+#pragma unroll
+          for (int c = 0; c < kTile; c += 32) tmem_wait_ld32(x + c);
+          const int hi = pos - j * kTile;                                     // columns 0 .. hi are seen
+          const int lo = p.window > 0 ? pos - p.window + 1 - j * kTile : 0;   // from column lo on
+          if (pos0 < (j + 1) * kTile - 1 || (p.window > 0 && pos0 + ntok - p.window > j * kTile)) {
+#pragma unroll
+            for (int c = 0; c < kTile; ++c) x[c] = c <= hi && c >= lo ? x[c] : 0xff800000u;  // -inf
+          }
+          float mx = __uint_as_float(x[0]);
+#pragma unroll
+          for (int c = 1; c < kTile; ++c) mx = fmaxf(mx, __uint_as_float(x[c]));
+          mx *= p.scale_log2e;
+          const bool first = j == w.j0[s];
+          const bool grow = mx > m + kSlack;  // also for the first value: m is -inf
+          if (__any_sync(0xffffffffu, grow)) {
+            const float w_old = grow ? fast_exp2(m - mx) : 1.f;
+            m = grow ? mx : m;
+            l *= w_old;
+            if (!first) {
+#pragma unroll
+              for (int c = 0; c < D; c += 32) {
+                uint32_t o[32];
+                tmem_ld32(t_o + c, o);
+                tmem_wait_ld32(o);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * w_old);
+                tmem_st32(t_o + c, o);
+              }
+            }
+          }
+          const float base = m == -INFINITY ? 0.f : m;
+          float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll
+          for (int c = 0; c < kTile; c += 2) {
+            const float a = fast_exp2(fmaf(__uint_as_float(x[c]), p.scale_log2e, -base));
+            const float b = fast_exp2(fmaf(__uint_as_float(x[c + 1]), p.scale_log2e, -base));
+            sum0 += a;
+            sum1 += b;
+            x[c / 2] = pack2<T>(a, b);
+          }
+          l += sum0 + sum1;
+#pragma unroll
+          for (int c = 0; c < kTile / 2; c += 32) tmem_st32(t_s + c, x + c);
+          tc_wait_st();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[s]);
+      }
+      // ---- the item's result
+      const bool has = w.j0[s] < w.j1[s];
+      if (has) {
+        wait(&o_full[s], o_round & 1);
+        ++o_round;
+        __syncwarp();
+        tc_fence_after();
+      }
+      const bool two = !w.dual && w.n > 1;  // two states of the same rows
+      float scale = 1.f, m_out = m, l_out = l;
+      if (two && s == 1) {
+        ml[row * 2] = m;
+        ml[row * 2 + 1] = l;
+      }
+      if (two) {
+        named_bar_sync(1, 256);
+        if (s == 0) {
+          const float m1 = ml[row * 2], l1 = ml[row * 2 + 1];
+          m_out = fmaxf(m, m1);
+          const float b = m_out == -INFINITY ? 0.f : m_out;
+          scale = fast_exp2(m - b);
+          l_out = l * scale + l1 * fast_exp2(m1 - b);
+        }
+      }
+      const int64_t tok = (int64_t)e.q_start + tok0 + tok_in;
+      const int64_t orow = tok * p.num_q_heads + w.it.kvh * g + head_in;
+      const bool split = e.nsplit > 1;
+      const int tile_rows = min(p.item_tokens, e.q_len) * g;
+      const int64_t prow = (int64_t)e.part_base +
+                           ((int64_t)(w.it.qtile * e.nsplit + w.it.split) * p.num_kv_heads + w.it.kvh) * tile_rows +
+                           (tok0 - w.it.tok0) * g + row;
+      const float inv = split ? 1.f : (l_out > 0.f ? 1.f / l_out : 0.f);
+      const bool writes = live && (w.dual || s == 0);
+      constexpr int kPart = D / 2;  // columns that go through the merge buffer at a time (the space of Q's second tile)
+      float *buf = reinterpret_cast<float *>(smem + C::kQBytes);
+#pragma unroll 1
+      for (int c0 = 0; c0 < D; c0 += kPart) {
+        if (two && s == 1) {
+          // stream 1's columns of this part, column by column (consecutive rows: no bank conflicts); stream 0 weights
+          if (warp_live) {
+#pragma unroll
+            for (int c = 0; c < kPart; c += 32) {
+              uint32_t o[32];
+              tmem_ld32(t_o + c0 + c, o);
+              tmem_wait_ld32(o);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) buf[(c + i) * kRows + row] = __uint_as_float(o[i]);
+            }
+          }
+          named_bar_sync(1, 256);
+          fence_proxy_async();  // the buffer's next use is by the loads
+          named_bar_sync(2, 256);
+          continue;
+        }
+        if (two) named_bar_sync(1, 256);
+        if (warp_live && (w.dual || s == 0)) {
+          const float s1 = two ? fast_exp2(ml[row * 2] - (m_out == -INFINITY ? 0.f : m_out)) : 0.f;
+#pragma unroll
+          for (int c = 0; c < kPart; c += 32) {
+            uint32_t o[32];
+            if (has) {
+              tmem_ld32(t_o + c0 + c, o);
+              tmem_wait_ld32(o);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = 0;
+            }
+            float f[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(o[i]);
+            if (two) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) f[i] = f[i] * scale + buf[(c + i) * kRows + row] * s1;
+            }
+            if (writes) {
+              if (split) {
+                float4 *dst = reinterpret_cast<float4 *>(p.part_o + prow * D + c0 + c);
+#pragma unroll
+                for (int i = 0; i < 32; i += 4) dst[i / 4] = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+              } else {
+                uint4 *dst = reinterpret_cast<uint4 *>(static_cast<T *>(p.out) + orow * D + c0 + c);
+#pragma unroll
+                for (int i = 0; i < 32; i += 8)
+                  dst[i / 8] = make_uint4(pack2<T>(f[i] * inv, f[i + 1] * inv), pack2<T>(f[i + 2] * inv, f[i + 3] * inv),
+                                          pack2<T>(f[i + 4] * inv, f[i + 5] * inv), pack2<T>(f[i + 6] * inv, f[i + 7] * inv));
+              }
+            }
+          }
+        }
+        if (two) {
+          fence_proxy_async();
+          named_bar_sync(2, 256);
+        }
+      }
+      // the merge buffer lies over Q's second tile: only now may the next item's rows come in
+      if (s == 1 && w.n > 0 && !w.dual && warp == 4 && lane == 0) mbar_arrive(q_empty);
+      if (writes) {
+        if (split) *reinterpret_cast<float2 *>(p.part_ml + prow * 2) = make_float2(m_out, l_out);
+        else if (p.lse != nullptr) p.lse[orow] = l_out > 0.f ? (m_out + log2f(l_out)) * kLn2 : -INFINITY;
+      }
+      tc_fence_before();  // the reads of O are ordered before the next item's products (which wait for its P)
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag) __nanosleep(1000000);  // copies that nothing has waited for land before the block's memory is given back
+  if (warp == 9) tmem_dealloc(tmem, 512);
+}
+
+// One warp per (token, q head) of the sequences that were split: the log-sum-exp merge in split order.
+template <typename T, int D, int N>
+__global__ void __launch_bounds__(256) chunk_merge_kernel(const __grid_constant__ ChunkParams p,
+                                                         const __grid_constant__ ChunkSeqs<N> seqs) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const ChunkSeq &e = seqs.s[blockIdx.y];
+  if (e.nsplit <= 1) return;
+  const int lane = threadIdx.x & 31;
+  const int64_t rows = (int64_t)e.q_len * p.num_q_heads;
+  constexpr int kCols = D / 32;
+  for (int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); w < rows; w += (int64_t)gridDim.x * 8) {
+    const int tok = (int)(w / p.num_q_heads), hq = (int)(w - (int64_t)tok * p.num_q_heads);
+    const int kvh = hq / p.group, h = hq - kvh * p.group;
+    const int qtile = tok / p.item_tokens;
+    const int tile_rows = min(p.item_tokens, e.q_len) * p.group;
+    const int64_t prow0 = (int64_t)e.part_base + ((int64_t)qtile * e.nsplit * p.num_kv_heads + kvh) * tile_rows +
+                          (tok - qtile * p.item_tokens) * p.group + h;
+    const int64_t step = (int64_t)p.num_kv_heads * tile_rows;
+    float m = -INFINITY;
+    for (int s = lane; s < e.nsplit; s += 32) m = fmaxf(m, __ldcg(p.part_ml + (prow0 + s * step) * 2));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float base = m == -INFINITY ? 0.f : m;
+    float l = 0.f, acc[kCols];
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) acc[c] = 0.f;
+    for (int s = 0; s < e.nsplit; ++s) {
+      const int64_t pr = prow0 + s * step;
+      const float2 v = __ldcg(reinterpret_cast<const float2 *>(p.part_ml + pr * 2));
+      const float f = fast_exp2(v.x - base);
+      l = fmaf(f, v.y, l);
+      const float *src = p.part_o + pr * D + lane * kCols;
+      if (kCols == 4) {
+        const float4 t = __ldcg(reinterpret_cast<const float4 *>(src));
+        acc[0] = fmaf(f, t.x, acc[0]); acc[1] = fmaf(f, t.y, acc[1]);
+        acc[2] = fmaf(f, t.z, acc[2]); acc[kCols - 1] = fmaf(f, t.w, acc[kCols - 1]);
+      } else {
+        const float2 t = __ldcg(reinterpret_cast<const float2 *>(src));
+        acc[0] = fmaf(f, t.x, acc[0]); acc[1] = fmaf(f, t.y, acc[1]);
+      }
+    }
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    const int64_t orow = ((int64_t)e.q_start + tok) * p.num_q_heads + hq;
+    uint32_t *dst = reinterpret_cast<uint32_t *>(static_cast<T *>(p.out) + orow * D + lane * kCols);
+#pragma unroll
+    for (int c = 0; c < kCols; c += 2) dst[c / 2] = pack2<T>(acc[c] * inv, acc[c + 1] * inv);
+    if (lane == 0 && p.lse != nullptr) p.lse[orow] = l > 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
+  }
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                                  const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn encode_fn() {
+  static EncodeTiledFn fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void *ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiledFn>(ptr);
+  });
+  return fn;
+}
+
+int encode(CUtensorMap *tm, const void *base, int32_t dtype, const cuuint64_t (&dims)[3], const cuuint64_t (&strides)[2],
+           const cuuint32_t (&box)[3]) {
+  EncodeTiledFn fn = encode_fn();
+  if (fn == nullptr) return fail(MSCO_ERR_CUDA, "chunk_attention: cuTensorMapEncodeTiled is not available");
+  const cuuint32_t one[3] = {1, 1, 1};
+  const CUresult r = fn(tm, dtype == MSCO_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+                        const_cast<void *>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(MSCO_ERR_CUDA, "chunk_attention: cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return MSCO_OK;
+}
+
+template <typename T, int D, int N>
+int launch_sized(const MscoChunkDesc &d, const ChunkParams &p, const ChunkSeq *src, int64_t q_rows, int sms,
+                 cudaStream_t stream) {
+  using C = Cfg<D>;
+  static_assert(C::kDynSmem <= 232448, "shared memory of one SM exceeded");
+  const cuuint64_t h = (cuuint64_t)d.num_kv_heads, bs = (cuuint64_t)d.block_size, nb = (cuuint64_t)d.num_blocks;
+  const cuuint32_t rows = (cuuint32_t)std::min(d.block_size, kTile);
+  CUtensorMap tq, tk, tv;
+  int rc = encode(&tq, p.q, d.q_dtype, {(cuuint64_t)D, (cuuint64_t)d.num_q_heads, (cuuint64_t)q_rows},
+                  {(cuuint64_t)D * 2, (cuuint64_t)d.num_q_heads * D * 2},
+                  {64u, (cuuint32_t)p.group, (cuuint32_t)(p.item_tokens / 2)});
+  if (rc != MSCO_OK) return rc;
+  for (int i = 0; i < 2; ++i) {
+    const void *cache = i == 0 ? p.key_cache : p.value_cache;
+    CUtensorMap *tm = i == 0 ? &tk : &tv;
+    rc = d.cache_layout == 1
+             ? encode(tm, cache, d.kv_dtype, {(cuuint64_t)D, bs, nb * h}, {(cuuint64_t)D * 2, bs * D * 2}, {64u, rows, 1u})
+             : encode(tm, cache, d.kv_dtype, {(cuuint64_t)D, h, nb * bs}, {(cuuint64_t)D * 2, h * D * 2}, {64u, 1u, rows});
+    if (rc != MSCO_OK) return rc;
+  }
+  ChunkSeqs<N> seqs;
+  bool split = false;
+  int64_t max_rows = 0;
+  for (int i = 0; i < p.nseq; ++i) {
+    seqs.s[i] = src[i];
+    if (src[i].nsplit > 1) {
+      split = true;
+      max_rows = std::max<int64_t>(max_rows, (int64_t)src[i].q_len * p.num_q_heads);
+    }
+  }
+  auto kfn = chunk_tc_kernel<T, D, N>;
+  // set per call: the attribute belongs to a device
+  MSCO_CUDA_CHECK(cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kDynSmem));
+  kfn<<<std::min(p.items, sms), kThreads, C::kDynSmem, stream>>>(tq, tk, tv, p, seqs);
+  MSCO_CUDA_CHECK(cudaGetLastError());
+  if (split) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)std::min<int64_t>((max_rows + 7) / 8, 1024), (unsigned)p.nseq);
+    cfg.blockDim = dim3(256);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    MSCO_CUDA_CHECK(cudaLaunchKernelEx(&cfg, chunk_merge_kernel<T, D, N>, p, seqs));
+  }
+  return MSCO_OK;
+}
+
+template <typename T, int D>
+int launch_typed(const MscoChunkDesc &d, const ChunkParams &p, const ChunkSeq *src, int64_t q_rows, int sms,
+                 cudaStream_t stream) {
+  if (p.nseq <= kChunkSeqsSmall) return launch_sized<T, D, kChunkSeqsSmall>(d, p, src, q_rows, sms, stream);
+  return launch_sized<T, D, kChunkSeqsMax>(d, p, src, q_rows, sms, stream);
+}
+
+}  // namespace
+
+// Pages have to tile a KV tile (or be tiled by it) in pieces of whole 8-row swizzle groups.
+bool chunk_tc_supported(const MscoChunkDesc &d) {
+  const int bs = d.block_size;
+  const bool bs_ok = bs % kTile == 0 || bs == 8 || bs == 16 || bs == 32 || bs == 64;
+  const int group = d.num_q_heads / d.num_kv_heads;
+  return (d.head_dim == 64 || d.head_dim == 128) && bs_ok && group <= kRows && d.kv_dtype == d.q_dtype && d.qk_scale > 0 &&
+         d.num_blocks * (int64_t)bs < (1ll << 31) && d.num_blocks * (int64_t)d.num_kv_heads < (1ll << 31);
+}
+
+int launch_chunk_tc(const MscoChunkDesc &d, const ChunkParams &p, const ChunkSeq *seqs, int64_t q_rows, int sms,
+                    cudaStream_t stream) {
+  const bool f16 = d.q_dtype == MSCO_DTYPE_F16;
+  if (d.head_dim == 64)
+    return f16 ? launch_typed<__half, 64>(d, p, seqs, q_rows, sms, stream)
+               : launch_typed<__nv_bfloat16, 64>(d, p, seqs, q_rows, sms, stream);
+  return f16 ? launch_typed<__half, 128>(d, p, seqs, q_rows, sms, stream)
+             : launch_typed<__nv_bfloat16, 128>(d, p, seqs, q_rows, sms, stream);
+}
+
+int chunk_tc_status() {
+  int v = 0;
+  if (cudaMemcpyFromSymbol(&v, g_chunk_error, sizeof(v)) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return MSCO_ERR_CUDA;
+  }
+  return v;
+}
+
+}  // namespace msco

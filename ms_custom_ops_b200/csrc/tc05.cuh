@@ -1,0 +1,96 @@
+// tcgen05 (5th-generation tensor core) wrappers of libmsco_b200.so: TMEM allocation, matrix instructions with
+// operands in shared memory or TMEM, moves between TMEM and registers.
+#pragma once
+
+#include <stdint.h>
+
+#include "msco_common.cuh"
+
+namespace msco {
+
+#ifdef __CUDACC__
+__device__ __forceinline__ void tmem_alloc(uint32_t *smem_dst, uint32_t cols) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(smem_dst)), "r"(cols)
+               : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc(uint32_t addr, uint32_t cols) {
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols) : "memory");
+}
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// arrives on the mbarrier once every matrix instruction that this thread has issued so far is complete
+__device__ __forceinline__ void tc_commit(uint64_t *bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+               : "memory");
+}
+
+// Shared-memory matrix descriptor, 128-byte swizzle.  K-major operand: rows of 128 bytes (64 16-bit elements of the
+// contraction), 8-row groups 1024 bytes apart (stride); the leading offset is not used.  MN-major operand: 64
+// elements of the free dimension per 128-byte row, rows along the contraction, 8-row groups 1024 bytes apart
+// (stride), the next 64 elements of the free dimension `leading` bytes on.
+__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t leading = 16) {
+  return (uint64_t)((addr & 0x3ffff) >> 4) | ((uint64_t)(leading >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+// Instruction descriptor of kind::f16 with float32 accumulators: M x N, A K-major, B K-major or MN-major.
+template <bool BF16, int M, int N, bool B_MN>
+__host__ __device__ constexpr uint32_t mma_idesc() {
+  return (1u << 4) | ((BF16 ? 1u : 0u) << 7) | ((BF16 ? 1u : 0u) << 10) | ((B_MN ? 1u : 0u) << 16) |
+         ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+// D (TMEM) = A (shared) * B (shared) (+ D); one thread issues
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
+      "r"((uint32_t)accumulate)
+      : "memory");
+}
+// D (TMEM) = A (TMEM, 16-bit pairs) * B (shared) (+ D)
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc),
+      "r"((uint32_t)accumulate)
+      : "memory");
+}
+
+// 32 columns of this warp's 32 TMEM lanes: lane i's row in its 32 registers
+#define MSCO_R4(r, i) "=r"((r)[i]), "=r"((r)[(i) + 1]), "=r"((r)[(i) + 2]), "=r"((r)[(i) + 3])
+#define MSCO_W4(r, i) "r"((r)[i]), "r"((r)[(i) + 1]), "r"((r)[(i) + 2]), "r"((r)[(i) + 3])
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t *r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,"
+      "%30,%31}, [%32];"
+      : MSCO_R4(r, 0), MSCO_R4(r, 4), MSCO_R4(r, 8), MSCO_R4(r, 12), MSCO_R4(r, 16), MSCO_R4(r, 20), MSCO_R4(r, 24),
+        MSCO_R4(r, 28)
+      : "r"(addr));
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t *r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,"
+      "%30,%31};" ::MSCO_W4(r, 0),
+      MSCO_W4(r, 4), MSCO_W4(r, 8), MSCO_W4(r, 12), MSCO_W4(r, 16), MSCO_W4(r, 20), MSCO_W4(r, 24), MSCO_W4(r, 28),
+      "r"(addr)
+      : "memory");
+}
+// Waits for this thread's loads from TMEM.  The registers pass through the statement: nothing that reads them can be
+// moved in front of it.
+#define MSCO_T4(r, i) "+r"((r)[i]), "+r"((r)[(i) + 1]), "+r"((r)[(i) + 2]), "+r"((r)[(i) + 3])
+__device__ __forceinline__ void tmem_wait_ld32(uint32_t *r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : MSCO_T4(r, 0), MSCO_T4(r, 4), MSCO_T4(r, 8), MSCO_T4(r, 12), MSCO_T4(r, 16), MSCO_T4(r, 20), MSCO_T4(r, 24),
+                 MSCO_T4(r, 28)
+               :
+               : "memory");
+}
+#undef MSCO_T4
+#undef MSCO_R4
+#undef MSCO_W4
+#endif  // __CUDACC__
+
+}  // namespace msco

@@ -146,6 +146,7 @@ class Chunk:
     def check(self, got=None, lse=None):
         if got is None:
             got, lse = self.run(return_lse=True)
+        ops.chunk_attention_check_status()
         tokens = sum(self.q_lens)
         out, want_lse, tol, lse_tol = self.expected()
         got = got[:tokens].double()
