@@ -38,117 +38,181 @@ __device__ __forceinline__ double weight_of(float p, float q) {
   return w > 0.0 ? w : 0.0;
 }
 
-template <typename T>
+constexpr int kLane = 16;            // vocabulary entries per lane and chunk
+constexpr int kChunk = 32 * kLane;   // entries of a chunk
+
+// Entries t0 .. t0 + 511 of a row, 16 per lane, 0 behind the end.  VEC: rows are 16-byte aligned (and t0 is a multiple of
+// 512), so a lane's entries come in 16-byte pieces, piece i of all lanes adjacent; otherwise one entry at a time.
+// The entry `skip` reads as 0.
+template <typename T, bool VEC>
+__device__ __forceinline__ void load_chunk(const T *row, int t0, int end, int lane, int skip, float (&x)[kLane]) {
+  if (VEC && t0 + kChunk <= end) {
+    constexpr int kPer = 16 / sizeof(T);
+#pragma unroll
+    for (int i = 0; i < kLane / kPer; ++i) {
+      const uint4 v = __ldg(reinterpret_cast<const uint4 *>(row + t0) + i * 32 + lane);
+      const T *e = reinterpret_cast<const T *>(&v);
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) x[i * kPer + k] = to_f32(e[k]);
+    }
+    if (skip >= t0 && skip < t0 + kChunk) {
+#pragma unroll
+      for (int i = 0; i < kLane; ++i)
+        if (t0 + (i / kPer * 32 + lane) * kPer + i % kPer == skip) x[i] = 0.f;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kLane; ++i) {
+      const int t = t0 + i * 32 + lane;
+      x[i] = t < end && t != skip ? to_f32(row[t]) : 0.f;
+    }
+  }
+}
+
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(kThreads) verify_kernel(VerifyArgs a) {
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = (int)cluster.block_rank(), ranks = (int)cluster.num_blocks();
   const int b = blockIdx.x / ranks;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   __shared__ double sums[kWarps];
-  __shared__ int s_taken;
   const T *target = static_cast<const T *>(a.target) + (int64_t)b * (a.drafts + 1) * a.vocab;
   const T *draft = static_cast<const T *>(a.draft);
   if (draft != nullptr) draft += (int64_t)b * a.drafts * a.vocab;
   const int32_t *dtok = a.draft_tokens + (int64_t)b * a.drafts;
   const float *u = a.uniform + (int64_t)b * (a.drafts + 1);
-  const int len = a.draft_lens != nullptr ? min(max(a.draft_lens[b], 0), a.drafts) : a.drafts;
-  if (warp == 0) {
-    int taken = 0;
-    for (int i0 = 0; i0 < len; i0 += 32) {
-      const int i = i0 + lane;
-      bool ok = false;
-      if (i < len) {
-        const int t = dtok[i];
-        if (t >= 0 && t < a.vocab) {
-          const double q = draft != nullptr ? (double)to_f32(draft[(int64_t)i * a.vocab + t]) : 1.0;
-          ok = (double)u[i] * q < (double)to_f32(target[(int64_t)i * a.vocab + t]);
-        }
+  const int len = a.draft_lens != nullptr ? min(max(__ldg(a.draft_lens + b), 0), a.drafts) : a.drafts;
+  // every warp finds the first draft that is turned down for itself: no exchange
+  int n = 0;
+  for (int i0 = 0; i0 < len; i0 += 32) {
+    const int i = i0 + lane;
+    bool ok = false;
+    if (i < len) {
+      const int t = __ldg(dtok + i);
+      if (t >= 0 && t < a.vocab) {
+        const double q = draft != nullptr ? (double)to_f32(draft[(int64_t)i * a.vocab + t]) : 1.0;
+        ok = (double)__ldg(u + i) * q < (double)to_f32(target[(int64_t)i * a.vocab + t]);
       }
-      const unsigned no = __ballot_sync(0xffffffffu, !ok);
-      taken += no != 0 ? __ffs(no) - 1 : 32;
-      if (no != 0) break;
     }
-    if (lane == 0) s_taken = min(taken, len);
+    const unsigned no = __ballot_sync(0xffffffffu, !ok);
+    n += no != 0 ? __ffs(no) - 1 : 32;
+    if (no != 0) break;
   }
-  __syncthreads();
-  const int n = s_taken;
+  n = min(n, len);
   const T *p = target + (int64_t)n * a.vocab;
   const bool rest = n < len;
   const T *q = rest && draft != nullptr ? draft + (int64_t)n * a.vocab : nullptr;
-  const int certain = rest && draft == nullptr ? dtok[n] : -1;  // a draft without probabilities was certain
-  // this warp's part of the vocabulary
-  const int per = (a.vocab + ranks * kWarps - 1) / (ranks * kWarps);
-  const int id = rank * kWarps + warp;
-  const int lo = (int)min((int64_t)a.vocab, (int64_t)id * per), hi = min(a.vocab, lo + per);
+  const int certain = rest && draft == nullptr ? __ldg(dtok + n) : -1;  // a draft without probabilities was certain
+  // this warp's part of the vocabulary: up to 32 chunks of `span` entries, lane k keeps the sum of chunk k
+  const int warps = ranks * kWarps, id = rank * kWarps + warp;
+  const int blocks = (a.vocab + kChunk - 1) / kChunk, per = (blocks + warps - 1) / warps;  // in units of kChunk
+  const int span = (per + 31) / 32 * kChunk;
+  const int lo = (int)min((int64_t)a.vocab, (int64_t)id * per * kChunk);
+  const int hi = (int)min((int64_t)a.vocab, (int64_t)lo + (int64_t)per * kChunk);
   int drawn = -1;
   bool here = false, found = false;
   for (int mode = 0; mode < 2; ++mode) {  // mode 1: the rest was nowhere positive, draw from the target itself
-    const bool less = mode == 0 && rest;
-    auto weight = [&](int t) -> double {
-      const float pt = to_f32(p[t]);
-      if (!less) return weight_of(pt, 0.f);
-      if (q != nullptr) return weight_of(pt, to_f32(q[t]));
-      return t == certain ? 0.0 : weight_of(pt, 0.f);
-    };
-    double s = 0.0;
-    for (int t = lo + lane; t < hi; t += 32) s += weight(t);
+    const bool less = mode == 0 && q != nullptr;
+    const int skip = mode == 0 ? certain : -1;
+    double mine = 0.0, s = 0.0;
+    for (int k = 0, c0 = lo; c0 < hi; ++k, c0 += span) {
+      double sum = 0.0;
+      for (int t0 = c0; t0 < min(hi, c0 + span); t0 += kChunk) {
+        float x[kLane], y[kLane];
+        load_chunk<T, VEC>(p, t0, hi, lane, skip, x);
+        if (less) {
+          load_chunk<T, VEC>(q, t0, hi, lane, -1, y);
+        } else {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+          for (int i = 0; i < kLane; ++i) y[i] = 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < kLane; ++i) sum += weight_of(x[i], y[i]);
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (lane == k) mine = sum;
+      s += sum;
+    }
     if (lane == 0) sums[warp] = s;
     cluster.sync();
     double total = 0.0, before = 0.0;
     for (int r = 0; r < ranks; ++r) {
       const double *rs = cluster.map_shared_rank(sums, r);
+#pragma unroll
       for (int w = 0; w < kWarps; ++w) {
         if (r * kWarps + w == id) before = total;
         total += rs[w];
       }
     }
     // every warp adds the sums in the same order, so all agree on the total and on whose part holds the border
-    const double goal = (double)u[a.drafts] * total;
+    const double goal = (double)__ldg(u + a.drafts) * total;
     found = goal >= 0.0 && goal < total;  // not for a row that is nowhere positive, nor for uniform outside [0, 1)
     here = found && before <= goal && before + s > goal;
     cluster.sync();  // the sums have been read
-    if (total > 0.0) {
-      if (here) {
-        double run = before;
-        int last = -1;
-        for (int t0 = lo; t0 < hi && drawn < 0; t0 += 32) {
-          const int t = t0 + lane;
-          const double w = t < hi ? weight(t) : 0.0;
-          double c = w;
+    if (!(total > 0.0)) continue;
+    if (here) {
+      // the chunk in which the running sum passes the goal, then the entry
+      double c = mine;
 #pragma unroll
-          for (int o = 1; o < 32; o <<= 1) {
-            const double up = __shfl_up_sync(0xffffffffu, c, o);
-            if (lane >= o) c += up;
-          }
-          const unsigned over = __ballot_sync(0xffffffffu, run + c > goal);
-          const unsigned pos = __ballot_sync(0xffffffffu, w > 0.0);
-          if (over != 0) drawn = t0 + __ffs(over) - 1;
-          if (pos != 0) last = t0 + 31 - __clz(pos);
-          run += __shfl_sync(0xffffffffu, c, 31);
-        }
-        // the part's sum and the scan round differently in the last place: the last entry that counts then
-        if (drawn < 0) drawn = last;
+      for (int o = 1; o < 32; o <<= 1) {
+        const double up = __shfl_up_sync(0xffffffffu, c, o);
+        if (lane >= o) c += up;
       }
-      break;
+      const unsigned over = __ballot_sync(0xffffffffu, before + c > goal);
+      // (sums taken in another order differ in the last place: the last chunk that counts then)
+      const unsigned some = __ballot_sync(0xffffffffu, mine > 0.0);
+      const int k = over != 0 ? __ffs(over) - 1 : 31 - __clz(some);
+      double run = before + (__shfl_sync(0xffffffffu, c, k) - __shfl_sync(0xffffffffu, mine, k));
+      int last = -1;
+      const int c0 = lo + k * span, c1 = min(hi, c0 + span);
+      for (int t0 = c0; t0 < c1 && drawn < 0; t0 += kChunk) {
+        double w[kLane], sum = 0.0;  // this lane's entries, consecutive ones
+        const int t = t0 + lane * kLane;
+#pragma unroll
+        for (int i = 0; i < kLane; ++i) {
+          const bool in = t + i < c1 && t + i != skip;
+          const float x = in ? to_f32(p[t + i]) : 0.f, y = in && less ? to_f32(q[t + i]) : 0.f;
+          w[i] = weight_of(x, y);
+          sum += w[i];
+        }
+        double d = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const double up = __shfl_up_sync(0xffffffffu, d, o);
+          if (lane >= o) d += up;
+        }
+        double at = run + (d - sum);
+        int hit = -1, end = -1;
+#pragma unroll
+        for (int i = 0; i < kLane; ++i) {
+          at += w[i];
+          if (hit < 0 && w[i] > 0.0 && at > goal) hit = t + i;
+          if (w[i] > 0.0) end = t + i;
+        }
+        const unsigned hits = __ballot_sync(0xffffffffu, hit >= 0), ends = __ballot_sync(0xffffffffu, end >= 0);
+        if (hits != 0) drawn = __shfl_sync(0xffffffffu, hit, __ffs(hits) - 1);
+        if (ends != 0) last = __shfl_sync(0xffffffffu, end, 31 - __clz(ends));
+        run += __shfl_sync(0xffffffffu, d, 31);
+      }
+      if (drawn < 0) drawn = last;
     }
+    break;
   }
   int32_t *out = a.tokens + (int64_t)b * (a.drafts + 1);
   if (here && lane == 0) out[n] = drawn;
   if (rank == 0 && warp == 0) {
     if (lane == 0) a.accepted[b] = n;
     for (int i = lane; i <= a.drafts; i += 32)
-      if (i != n || !found) out[i] = i < n ? dtok[i] : -1;
+      if (i != n || !found) out[i] = i < n ? __ldg(dtok + i) : -1;
   }
 }
 
 template <typename T>
 int launch_verify(const VerifyArgs &a, cudaStream_t st) {
-  // parts of at least 2048 entries per CTA
-  const int cluster = std::max(1, std::min(kMaxCluster, a.vocab / 2048));
+  // as many CTAs as have a chunk for each of their warps
   int c = 1;
-  while (c * 2 <= cluster) c *= 2;
+  while (c < kMaxCluster && (int64_t)c * kWarps * kChunk < a.vocab) c *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a.batch * c));
   cfg.blockDim = dim3(kThreads);
@@ -160,7 +224,12 @@ int launch_verify(const VerifyArgs &a, cudaStream_t st) {
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  MSCO_CUDA_CHECK(cudaLaunchKernelEx(&cfg, verify_kernel<T>, a));
+  const uintptr_t rows = reinterpret_cast<uintptr_t>(a.target) | reinterpret_cast<uintptr_t>(a.draft) |
+                         (uintptr_t)((int64_t)a.vocab * sizeof(T));
+  if ((rows & 15) == 0)
+    MSCO_CUDA_CHECK(cudaLaunchKernelEx(&cfg, verify_kernel<T, true>, a));
+  else
+    MSCO_CUDA_CHECK(cudaLaunchKernelEx(&cfg, verify_kernel<T, false>, a));
   return MSCO_OK;
 }
 

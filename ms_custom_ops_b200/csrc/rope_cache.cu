@@ -103,6 +103,149 @@ __global__ void __launch_bounds__(256) rope_cache_any_kernel(RopeArgs a) {
   }
 }
 
+// eight consecutive 16-bit values
+template <typename T>
+__device__ __forceinline__ void unpack8(const uint4 &v, float (&x)[8]) {
+  const T *e = reinterpret_cast<const T *>(&v);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = to_f32(e[i]);
+}
+__device__ __forceinline__ uint4 load_stream(const void *p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+
+// head_dim 64 / 128 / 256, 16-byte rows.  D / 8 lanes own a head row, eight consecutive elements each; such a group takes
+// ROWS consecutive head rows of one token, so the cosines and sines are fetched once for them and all ROWS loads are in
+// flight before the first is used.  The other element of a pair is in the same lane (interleaved) or rotary / 16 lanes on.
+template <typename T, int D, bool I8, bool INTER, bool NORM, int ROWS>
+__global__ void __launch_bounds__(256) rope_cache_vec_kernel(RopeArgs a) {
+  constexpr int L = D / 8;
+  const int sub = threadIdx.x & (L - 1);
+  const int rows = a.q_heads + 2 * a.kv_heads;
+  const int chunks = (rows + ROWS - 1) / ROWS;
+  const int64_t group = ((int64_t)blockIdx.x * 256 + threadIdx.x) / L;
+  const int64_t t_raw = group / chunks;
+  const bool in = t_raw < a.tokens;  // lanes behind the last token go along (shuffles), and store nothing
+  const int64_t t = in ? t_raw : a.tokens - 1;
+  const int r0 = (int)(group - t_raw * chunks) * ROWS;
+  const int d0 = sub * 8;
+  uint4 raw[ROWS];
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    const int r = min(r0 + i, rows - 1);
+    const T *src = r < a.q_heads ? static_cast<const T *>(a.q) + t * a.q_stride + (int64_t)r * D
+                   : r < a.q_heads + a.kv_heads
+                       ? static_cast<const T *>(a.k) + t * a.k_stride + (int64_t)(r - a.q_heads) * D
+                       : static_cast<const T *>(a.v) + t * a.v_stride + (int64_t)(r - a.q_heads - a.kv_heads) * D;
+    raw[i] = load_stream(src + d0);
+  }
+  const int32_t pos = __ldg(a.positions + t);
+  const int64_t slot = __ldg(a.slots + t);
+  const bool pos_ok = pos >= 0 && pos < a.max_positions;
+  const bool store = slot >= 0 && slot < a.slots_total && pos_ok;
+  if (in && r0 == 0 && sub == 0 && a.oob != nullptr && (!pos_ok || slot >= a.slots_total)) atomicAdd(a.oob, 1);
+  const int half = a.rotary >> 1;
+  const bool turns = d0 < a.rotary;
+  const bool first = INTER || d0 < half;
+  float c[8], sn[8];  // INTER: four pairs
+  {
+    const float *cs = a.cos_sin + (int64_t)(pos_ok ? pos : 0) * a.rotary;
+    const int i0 = INTER ? d0 >> 1 : (first ? d0 : d0 - half);
+    constexpr int kN = INTER ? 4 : 8;
+#pragma unroll
+    for (int i = 0; i < kN; i += 4) {
+      const float4 cc = turns && pos_ok ? __ldg(reinterpret_cast<const float4 *>(cs + i0 + i)) : make_float4(1, 1, 1, 1);
+      c[i] = cc.x; c[i + 1] = cc.y; c[i + 2] = cc.z; c[i + 3] = cc.w;
+      const float4 ss = turns && pos_ok ? __ldg(reinterpret_cast<const float4 *>(cs + half + i0 + i)) : make_float4(0, 0, 0, 0);
+      sn[i] = ss.x; sn[i + 1] = ss.y; sn[i + 2] = ss.z; sn[i + 3] = ss.w;
+    }
+  }
+  const int lane = threadIdx.x & 31;
+  const int other = turns ? (first ? lane + half / 8 : lane - half / 8) : lane;
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    const int r = r0 + i;
+    const int kind = r < a.q_heads ? 0 : (r < a.q_heads + a.kv_heads ? 1 : 2);
+    const int h = kind == 0 ? r : (kind == 1 ? r - a.q_heads : r - a.q_heads - a.kv_heads);
+    float x[8];
+    unpack8<T>(raw[i], x);
+    if (NORM) {
+      float ss = 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) ss = fmaf(x[k], x[k], ss);
+#pragma unroll
+      for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      const T *weight = static_cast<const T *>(kind == 0 ? a.q_weight : a.k_weight);
+      if (kind != 2 && weight != nullptr) {
+        const float inv = 1.f / sqrtf(ss * (1.f / D) + a.eps);
+        float w[8];
+        unpack8<T>(__ldg(reinterpret_cast<const uint4 *>(weight + d0)), w);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[k] = x[k] * inv * w[k];
+      }
+    }
+    float y[8];
+    if (INTER) {
+#pragma unroll
+      for (int k = 0; k < 8; k += 2) {
+        y[k] = x[k] * c[k / 2] - x[k + 1] * sn[k / 2];
+        y[k + 1] = x[k + 1] * c[k / 2] + x[k] * sn[k / 2];
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float o = __shfl_sync(0xffffffffu, x[k], other);
+        y[k] = first ? x[k] * c[k] - o * sn[k] : x[k] * c[k] + o * sn[k];
+      }
+    }
+    if (!in || r >= rows) continue;
+    if (kind == 2) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) y[k] = x[k];
+    }
+    const uint4 packed = make_uint4(pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3]), pack2<T>(y[4], y[5]), pack2<T>(y[6], y[7]));
+    if (kind == 0) {
+      T *dst = static_cast<T *>(a.q_out) + (t * a.q_heads + h) * D + d0;
+      *reinterpret_cast<uint4 *>(dst) = pos_ok ? packed : make_uint4(0, 0, 0, 0);
+    } else if (store) {
+      const int64_t at = cache_row(a, slot, h) + d0;
+      void *cache = kind == 1 ? a.k_cache : a.v_cache;
+      if (I8) {
+        const float *ds = (kind == 1 ? a.k_descale : a.v_descale) + h * D + d0;
+        const int32_t *of = kind == 1 ? a.k_offset : a.v_offset;
+        uint32_t q8[2] = {0, 0};
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float off = of != nullptr ? (float)__ldg(of + h * D + d0 + k) : 0.f;
+          q8[k / 4] |= (uint32_t)(uint8_t)quantise(y[k], __ldg(ds + k), off) << (8 * (k & 3));
+        }
+        *reinterpret_cast<uint2 *>(static_cast<int8_t *>(cache) + at) = make_uint2(q8[0], q8[1]);
+      } else {
+        *reinterpret_cast<uint4 *>(static_cast<T *>(cache) + at) = kind == 2 ? raw[i] : packed;
+      }
+    }
+  }
+}
+
+template <typename T, int D, bool I8, bool INTER, bool NORM>
+int launch_vec(const RopeArgs &a, cudaStream_t st) {
+  const int rows = a.q_heads + 2 * a.kv_heads;
+  constexpr int L = D / 8;
+  auto blocks_of = [&](int per) { return (a.tokens * ((rows + per - 1) / per) * L + 255) / 256; };
+  // four rows per group once that still fills the GPU several times over, one row where latency counts
+  if (blocks_of(4) >= 148 * 8) {
+    const int64_t blocks = blocks_of(4);
+    if (blocks > 0x7fffffffLL) return fail(MSCO_ERR_INVALID_ARG, "rope_and_cache: too many rows");
+    rope_cache_vec_kernel<T, D, I8, INTER, NORM, 4><<<(unsigned)blocks, 256, 0, st>>>(a);
+  } else {
+    rope_cache_vec_kernel<T, D, I8, INTER, NORM, 1><<<(unsigned)blocks_of(1), 256, 0, st>>>(a);
+  }
+  MSCO_CUDA_CHECK(cudaGetLastError());
+  return MSCO_OK;
+}
+
 template <typename T, bool I8>
 int launch_any(const RopeArgs &a, cudaStream_t st) {
   const int64_t warps = a.tokens * (a.q_heads + 2 * a.kv_heads);
@@ -110,6 +253,28 @@ int launch_any(const RopeArgs &a, cudaStream_t st) {
   rope_cache_any_kernel<T, I8><<<(unsigned)blocks, 256, 0, st>>>(a);
   MSCO_CUDA_CHECK(cudaGetLastError());
   return MSCO_OK;
+}
+
+template <typename T, int D, bool I8>
+int launch_vec_of(const RopeArgs &a, cudaStream_t st) {
+  const bool norm = a.q_weight != nullptr || a.k_weight != nullptr;
+  if (a.interleaved) return norm ? launch_vec<T, D, I8, true, true>(a, st) : launch_vec<T, D, I8, true, false>(a, st);
+  return norm ? launch_vec<T, D, I8, false, true>(a, st) : launch_vec<T, D, I8, false, false>(a, st);
+}
+
+// 16-byte pieces: every row address, and pairs that stay inside a lane or lie whole lanes apart
+template <typename T, bool I8>
+int launch_rope(const RopeArgs &a, cudaStream_t st) {
+  const uintptr_t all = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) |
+                        reinterpret_cast<uintptr_t>(a.q_out) | reinterpret_cast<uintptr_t>(a.k_cache) |
+                        reinterpret_cast<uintptr_t>(a.v_cache) | reinterpret_cast<uintptr_t>(a.cos_sin) |
+                        reinterpret_cast<uintptr_t>(a.q_weight) | reinterpret_cast<uintptr_t>(a.k_weight);
+  const bool strides = a.tokens == 1 || ((a.q_stride | a.k_stride | a.v_stride) & 7) == 0;
+  const bool vec = (all & 15) == 0 && strides && a.rotary % (a.interleaved ? 8 : 16) == 0;
+  if (vec && a.head_dim == 128) return launch_vec_of<T, 128, I8>(a, st);
+  if (vec && a.head_dim == 64) return launch_vec_of<T, 64, I8>(a, st);
+  if (vec && a.head_dim == 256) return launch_vec_of<T, 256, I8>(a, st);
+  return launch_any<T, I8>(a, st);
 }
 
 }  // namespace
@@ -162,6 +327,6 @@ extern "C" int msco_rope_and_cache(const MscoRopeDesc *desc, const void *query, 
   a.block_size = d.block_size; a.layout = d.cache_layout; a.interleaved = d.interleaved != 0; a.eps = d.eps;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool f16 = d.dtype == MSCO_DTYPE_F16;
-  if (i8) return f16 ? launch_any<__half, true>(a, st) : launch_any<__nv_bfloat16, true>(a, st);
-  return f16 ? launch_any<__half, false>(a, st) : launch_any<__nv_bfloat16, false>(a, st);
+  if (i8) return f16 ? launch_rope<__half, true>(a, st) : launch_rope<__nv_bfloat16, true>(a, st);
+  return f16 ? launch_rope<__half, false>(a, st) : launch_rope<__nv_bfloat16, false>(a, st);
 }
