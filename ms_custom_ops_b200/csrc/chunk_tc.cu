@@ -11,8 +11,8 @@
 // more than kSlack (a factor 256): until then P is up to 256 instead of 1, which costs no precision in a floating
 // format, and O stays where it is; it is rescaled in TMEM by the softmax warps in the rare tiles where it must.
 //
-// Warps: 0-3 / 4-7 softmax of stream 0 / 1, 8 loads (TMA, 128-byte swizzle), 9 matrix instructions (10, 11 idle: registers
-// are handed out by groups of four warps).
+// Warps: 0 loads (TMA, 128-byte swizzle), 1 matrix instructions (2, 3 idle: registers are handed out by groups of four
+// warps), 4-7 / 8-11 softmax of stream 0 / 1.
 // The matrix instructions are issued O_0 += P_0 V, S_0 = Q_0 K', O_1 += P_1 V, S_1 = Q_1 K' (K' the next tile); they execute in
 // that order, so a completed S' means that the product that read P, which lies over it, is complete too.
 #include <cuda.h>
@@ -31,6 +31,7 @@ constexpr int kRows = 128;        // rows of one stream
 constexpr int kTile = kChunkKvTile;
 constexpr int kThreads = 384;
 constexpr float kSlack = 8.f;     // log2 of how far a probability may exceed 1
+constexpr int kPart0 = 96;        // tokens of a tile whose probabilities are handed over first
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr uint32_t kWaitLimit = 1u << 22;
 
@@ -46,7 +47,7 @@ struct Cfg {
   static constexpr int kStages = D == 128 ? 5 : 10;
   static constexpr int kOffKv = 2 * kQBytes;
   static constexpr int kOffBar = kOffKv + kStages * kStageBytes;
-  static constexpr int kNumBars = 2 * kStages + 10;
+  static constexpr int kNumBars = 2 * kStages + 12;
   static constexpr int kOffMl = kOffBar + kNumBars * 8 + 16;  // [128][2] floats of the merge of the streams
   static constexpr int kSmem = kOffMl + kRows * 2 * 4;
   static constexpr int kDynSmem = kSmem + 1024;
@@ -58,13 +59,16 @@ struct Cfg {
 // stays inside their buffers, the result is worthless and the device's error word says so.
 struct Waiter {
   volatile int *abort;
-  __device__ __forceinline__ void operator()(uint64_t *bar, uint32_t parity) const {
-    for (uint32_t i = 0; i < kWaitLimit; ++i) {
-      if (mbar_try_wait(bar, parity)) return;
-      if (*abort) return;
+  __device__ __forceinline__ void operator()(uint64_t *bar, uint32_t parity) const {  // by a whole warp
+    for (uint32_t i = 0; !mbar_try_wait(bar, parity); ++i) {
+      if ((i & 255) != 255) continue;
+      if (*abort) break;
+      if (i >= kWaitLimit) {
+        *abort = 1;
+        atomicExch(&g_chunk_error, MSCO_ERR_TIMEOUT);
+      }
     }
-    *abort = 1;
-    atomicExch(&g_chunk_error, MSCO_ERR_TIMEOUT);
+    __syncwarp();
   }
 };
 
@@ -124,7 +128,8 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   uint64_t *bars = reinterpret_cast<uint64_t *>(smem + C::kOffBar);
   uint64_t *kv_full = bars, *kv_empty = bars + C::kStages;
   uint64_t *q_full = bars + 2 * C::kStages, *q_empty = q_full + 1, *s_full = q_full + 2, *p_full = q_full + 4,
-           *o_full = q_full + 6, *tail = q_full + 8, *fin = q_full + 9;
+           *o_full = q_full + 6, *tail = q_full + 8, *fin = q_full + 9,
+           *p_rest = q_full + 10;
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + C::kNumBars);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
   float *ml = reinterpret_cast<float *>(smem + C::kOffMl);
@@ -140,6 +145,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     for (int s = 0; s < 2; ++s) {
       mbar_init(&s_full[s], 1);
       mbar_init(&p_full[s], 4);
+      mbar_init(&p_rest[s], 4);
       mbar_init(&o_full[s], 1);
     }
     mbar_init(tail, 1);
@@ -147,7 +153,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     *abort_flag = 0;
     fence_barrier_init();
   }
-  if (warp == 9) tmem_alloc(tmem_slot, 512);
+  if (warp == 1) tmem_alloc(tmem_slot, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -155,9 +161,9 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   const Waiter wait{abort_flag};
   const int half = p.item_tokens >> 1;
 
-  // Registers: 384 x 168 at launch = 256 x 208 (softmax) + 128 x 88 (the other four warps, two of them idle)
-  if (warp >= 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-  if (warp == 8) {
+  // Registers: 384 x 168 at launch = 256 x 208 (softmax) + 128 x 88 (the first four warps)
+  if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+  if (warp == 0) {
     // ------------------------------------------------------------------ loads
     if (lane == 0) {
       prefetch_tmap(&tm_q);
@@ -191,7 +197,6 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         const uint32_t st = c % C::kStages, use = c / C::kStages;
         ++c;
         if (use > 0) wait(&kv_empty[st], (use - 1) & 1);
-        __syncwarp();
         uint8_t *dst = smem + C::kOffKv + st * C::kStageBytes;
         const int tok = j * kTile;
         const int a = max(0, alive0 - tok), b = min(kTile, alive1 - tok);  // rows of the tile that are alive
@@ -224,7 +229,6 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         if (patch) {
           wait(tail, tails & 1);
           ++tails;
-          __syncwarp();
           for (int i = lane; i < kTile * 8 * C::kBoxes; i += 32) {  // 16-byte pieces; a row is 128 bytes of a sub-tile
             const int x = i / (kTile * 8), row = (i / 8) % kTile;
             if (row < a || row >= b)
@@ -243,37 +247,49 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         if (i + ahead < w.n) load(&tm_k, w.it.tile0 + i + ahead, false);
       }
     }
-  } else if (warp == 9) {
+  } else if (warp == 1) {
     // ------------------------------------------------------------------ matrix instructions
-    if (lane == 0) {
+    // The whole warp goes through the loop, so that addresses and descriptors stay in uniform registers; one elected lane
+    // issues.
+    {
       constexpr uint32_t kIdQk = mma_idesc<kBf16, kRows, kTile, false>();
       constexpr uint32_t kIdPv = mma_idesc<kBf16, kRows, D, true>();
       const uint32_t q_addr = smem_u32(smem), kv_addr = smem_u32(smem + C::kOffKv);
-      uint32_t c = 0, q_round = 0, p_round[2] = {0, 0};
+      uint32_t c = 0, q_round = 0, p_par = 0;  // bit s: parity of stream s's next P
+      auto commit = [&](uint64_t *bar) {
+        if (elect_one()) tc_commit(bar);
+      };
       for (int r = 0, item = item_of(0); item < p.items; item = item_of(++r)) {
         const Work w = make_work(seqs, p, item);
         if (w.n == 0) continue;
         wait(q_full, q_round & 1);
         ++q_round;
         auto qk = [&](int s, uint32_t st) {
-          uint64_t a = smem_desc(q_addr + (w.dual ? s * C::kQBytes : 0)), b = smem_desc(kv_addr + st * C::kStageBytes);
-          asm volatile("" : "+l"(a), "+l"(b));  // the eight descriptors are one addition each, not values to keep
+          const uint64_t a = smem_desc(q_addr + (w.dual ? s * C::kQBytes : 0)), b = smem_desc(kv_addr + st * C::kStageBytes);
+          if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            const uint32_t off = ((k / 4) * (kRows * 128) + (k % 4) * 32) >> 4;
-            mma_ss(tmem + s * kTile, a + off, b + off, kIdQk, k > 0);
+            for (int k = 0; k < D / 16; ++k) {
+              const uint32_t off = ((k / 4) * (kRows * 128) + (k % 4) * 32) >> 4;
+              mma_ss(tmem + s * kTile, a + off, b + off, kIdQk, k > 0);
+            }
+            tc_commit(&s_full[s]);
           }
-          tc_commit(&s_full[s]);
         };
         auto pv = [&](int s, uint32_t st, bool acc) {
-          wait(&p_full[s], p_round[s] & 1);
-          ++p_round[s];
+          const uint64_t b = smem_desc(kv_addr + st * C::kStageBytes, C::kSub);
+          wait(&p_full[s], (p_par >> s) & 1);
           tc_fence_after();
-          uint64_t b = smem_desc(kv_addr + st * C::kStageBytes, C::kSub);
-          asm volatile("" : "+l"(b));
+          if (elect_one())
 #pragma unroll
-          for (int k = 0; k < kTile / 16; ++k)
-            mma_ts(tmem + C::kColO + s * D, tmem + s * kTile + k * 8, b + (k * 2048 >> 4), kIdPv, acc || k > 0);
+            for (int k = 0; k < kPart0 / 16; ++k)
+              mma_ts(tmem + C::kColO + s * D, tmem + s * kTile + k * 8, b + (k * 2048 >> 4), kIdPv, acc || k > 0);
+          wait(&p_rest[s], (p_par >> s) & 1);
+          p_par ^= 1u << s;
+          tc_fence_after();
+          if (elect_one())
+#pragma unroll
+            for (int k = kPart0 / 16; k < kTile / 16; ++k)
+              mma_ts(tmem + C::kColO + s * D, tmem + s * kTile + k * 8, b + (k * 2048 >> 4), kIdPv, true);
         };
         auto take = [&]() {  // the next stage of the ring, filled
           const uint32_t st = c % C::kStages;
@@ -287,51 +303,51 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
             // V of tile j, then K of tile j + 1; the streams alternate
             const bool has_v = j >= w.it.tile0, has_k = j + 1 < w.it.tile1;
             const uint32_t sv = has_v ? take() : 0, sk = has_k ? take() : 0;
-#pragma unroll 1
+#pragma unroll
             for (int s = 0; s < 2; ++s) {
               if (has_v && j >= w.j0[s] && j < w.j1[s]) {
                 pv(s, sv, j > w.j0[s]);
-                if (j + 1 == w.j1[s]) tc_commit(&o_full[s]);
+                if (j + 1 == w.j1[s]) commit(&o_full[s]);
               }
-              if (s == 1 && has_v) tc_commit(&kv_empty[sv]);
+              if (s == 1 && has_v) commit(&kv_empty[sv]);
               if (has_k && j + 1 >= w.j0[s] && j + 1 < w.j1[s]) qk(s, sk);
             }
             if (has_k) {
-              tc_commit(&kv_empty[sk]);
-              if (j + 2 >= w.it.tile1) tc_commit(q_empty);
+              commit(&kv_empty[sk]);
+              if (j + 2 >= w.it.tile1) commit(q_empty);
             }
           }
         } else {
           for (int i = 0; i < min(2, w.n); ++i) {
             const uint32_t st = take();
             qk(i, st);
-            tc_commit(&kv_empty[st]);
-            if (i + 1 == w.n) tc_commit(q_empty);
+            commit(&kv_empty[st]);
+            if (i + 1 == w.n) commit(q_empty);
           }
           for (int i = 0; i < w.n; ++i) {
             const int s = i & 1;
             const uint32_t sv = take();
             pv(s, sv, i > 1);
-            tc_commit(&kv_empty[sv]);
+            commit(&kv_empty[sv]);
             if (i + 2 >= w.n) {
-              tc_commit(&o_full[s]);
+              commit(&o_full[s]);
               continue;
             }
             const uint32_t sk = take();
             qk(s, sk);
-            tc_commit(&kv_empty[sk]);
-            if (i + 3 == w.n) tc_commit(q_empty);
+            commit(&kv_empty[sk]);
+            if (i + 3 == w.n) commit(q_empty);
           }
         }
       }
-      tc_commit(fin);  // every arrival that the instructions still owe has happened before the block ends
+      commit(fin);  // every arrival that the instructions still owe has happened before the block ends
       wait(fin, 0);
     }
     __syncwarp();
-  } else if (warp < 8) {
+  } else if (warp >= 4) {
     // ------------------------------------------------------------------ softmax, one row per thread
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-    const int s = warp >> 2;
+    const int s = (warp >> 2) - 1;
     const int row = threadIdx.x & 127;
     const uint32_t lanes = (uint32_t)(warp & 3) * 32 << 16;
     const uint32_t t_s = tmem + lanes + s * kTile, t_o = tmem + lanes + C::kColO + s * D;
@@ -347,18 +363,18 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       const bool warp_live = __any_sync(0xffffffffu, live);
       const int pos0 = e.ctx - e.q_len + tok0;
       const int pos = live ? pos0 + tok_in : -1;
+      const int j_beg = s == 0 ? w.j0[0] : w.j0[1], j_end = s == 0 ? w.j1[0] : w.j1[1];
       float m = -INFINITY, l = 0.f;
-      if (warp == 4 && w.n > 0) {
+      if (warp == 8 && w.n > 0) {
         // One of the two arrivals that free Q's space is stream 1's: at once (dual), or when the merge is through with it
         // (single).  It comes behind the arrival of the item's rows, so never before the one of the item in front.
         wait(q_full, q_round & 1);
         ++q_round;
         if (w.dual && lane == 0) mbar_arrive(q_empty);
       }
-      for (int j = w.j0[s]; j < w.j1[s]; j += w.step) {
+      for (int j = j_beg; j < j_end; j += w.step) {
         wait(&s_full[s], s_round & 1);
         ++s_round;
-        __syncwarp();
         tc_fence_after();
         if (warp_live) {
           uint32_t x[kTile];
@@ -372,11 +388,19 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
 #pragma unroll
             for (int c = 0; c < kTile; ++c) x[c] = c <= hi && c >= lo ? x[c] : 0xff800000u;  // -inf
           }
-          float mx = __uint_as_float(x[0]);
+          // four chains of three-way maxima: one chain would be 128 dependent steps
+          float mx4[4];
 #pragma unroll
-          for (int c = 1; c < kTile; ++c) mx = fmaxf(mx, __uint_as_float(x[c]));
-          mx *= p.scale_log2e;
-          const bool first = j == w.j0[s];
+          for (int i = 0; i < 4; ++i) mx4[i] = __uint_as_float(x[i]);
+#pragma unroll
+          for (int c = 4; c < kTile - 4; c += 8)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              mx4[i] = fmaxf(mx4[i], fmaxf(__uint_as_float(x[c + i]), __uint_as_float(x[c + 4 + i])));
+#pragma unroll
+          for (int i = 0; i < 4; ++i) mx4[i] = fmaxf(mx4[i], __uint_as_float(x[kTile - 4 + i]));
+          const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * p.scale_log2e;
+          const bool first = j == j_beg;
           const bool grow = mx > m + kSlack;  // also for the first value: m is -inf
           if (__any_sync(0xffffffffu, grow)) {
             const float w_old = grow ? fast_exp2(m - mx) : 1.f;
@@ -395,30 +419,45 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
             }
           }
           const float base = m == -INFINITY ? 0.f : m;
-          float sum0 = 0.f, sum1 = 0.f;
+          const uint64_t scale2 = pack_f32x2(p.scale_log2e, p.scale_log2e), base2 = pack_f32x2(-base, -base);
+          uint64_t sum2[2] = {0, 0};
 #pragma unroll
-          for (int c = 0; c < kTile; c += 2) {
-            const float a = fast_exp2(fmaf(__uint_as_float(x[c]), p.scale_log2e, -base));
-            const float b = fast_exp2(fmaf(__uint_as_float(x[c + 1]), p.scale_log2e, -base));
-            sum0 += a;
-            sum1 += b;
-            x[c / 2] = pack2<T>(a, b);
+          for (int c0 = 0; c0 < kTile; c0 += 32) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              const uint64_t v = fma_f32x2(pack_f32x2(__uint_as_float(x[c0 + i]), __uint_as_float(x[c0 + i + 1])), scale2, base2);
+              float a, b;
+              unpack_f32x2(v, a, b);
+              a = fast_exp2(a);
+              b = fast_exp2(b);
+              sum2[(i >> 1) & 1] = add_f32x2(sum2[(i >> 1) & 1], pack_f32x2(a, b));
+              pk[i / 2] = pack2<T>(a, b);
+            }
+            tmem_st16(t_s + c0 / 2, pk);
+            if (c0 + 32 == kPart0) {  // the product may start on these tokens
+              tc_wait_st();
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&p_full[s]);
+            }
           }
-          l += sum0 + sum1;
-#pragma unroll
-          for (int c = 0; c < kTile / 2; c += 32) tmem_st32(t_s + c, x + c);
           tc_wait_st();
+          float s0, s1;
+          unpack_f32x2(add_f32x2(sum2[0], sum2[1]), s0, s1);
+          l += s0 + s1;
+        } else if (lane == 0) {
+          mbar_arrive(&p_full[s]);
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[s]);
+        if (lane == 0) mbar_arrive(&p_rest[s]);
       }
       // ---- the item's result
-      const bool has = w.j0[s] < w.j1[s];
+      const bool has = j_beg < j_end;
       if (has) {
         wait(&o_full[s], o_round & 1);
         ++o_round;
-        __syncwarp();
         tc_fence_after();
       }
       const bool two = !w.dual && w.n > 1;  // two states of the same rows
@@ -508,7 +547,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         }
       }
       // the merge buffer lies over Q's second tile: only now may the next item's rows come in
-      if (s == 1 && w.n > 0 && !w.dual && warp == 4 && lane == 0) mbar_arrive(q_empty);
+      if (warp == 8 && w.n > 0 && !w.dual && lane == 0) mbar_arrive(q_empty);
       if (writes) {
         if (split) *reinterpret_cast<float2 *>(p.part_ml + prow * 2) = make_float2(m_out, l_out);
         else if (p.lse != nullptr) p.lse[orow] = l_out > 0.f ? (m_out + log2f(l_out)) * kLn2 : -INFINITY;
@@ -519,7 +558,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   tc_fence_before();
   __syncthreads();
   if (*abort_flag) __nanosleep(1000000);  // copies that nothing has waited for land before the block's memory is given back
-  if (warp == 9) tmem_dealloc(tmem, 512);
+  if (warp == 1) tmem_dealloc(tmem, 512);
 }
 
 // One warp per (token, q head) of the sequences that were split: the log-sum-exp merge in split order.
