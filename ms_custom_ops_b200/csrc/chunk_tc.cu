@@ -31,7 +31,6 @@ constexpr int kRows = 128;        // rows of one stream
 constexpr int kTile = kChunkKvTile;
 constexpr int kThreads = 384;
 constexpr float kSlack = 8.f;     // log2 of how far a probability may exceed 1
-constexpr int kPart0 = 96;        // tokens of a tile whose probabilities are handed over first
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr uint32_t kWaitLimit = 1u << 22;
 
@@ -45,12 +44,16 @@ struct Cfg {
   static constexpr int kStageBytes = kTile * D * 2;
   static constexpr int kQBytes = kRows * D * 2;
   static constexpr int kStages = D == 128 ? 5 : 10;
+  // tokens of a tile whose probabilities are handed over first (kTile: all at once)
+  static constexpr int kPart0 = D == 128 ? 96 : kTile;
   static constexpr int kOffKv = 2 * kQBytes;
   static constexpr int kOffBar = kOffKv + kStages * kStageBytes;
   static constexpr int kNumBars = 2 * kStages + 12;
   static constexpr int kOffMl = kOffBar + kNumBars * 8 + 16;  // [128][2] floats of the merge of the streams
   static constexpr int kSmem = kOffMl + kRows * 2 * 4;
   static constexpr int kDynSmem = kSmem + 1024;
+  // of eight pairs of probabilities, those that are computed by the FMA pipe
+  static constexpr int kPolyOf8 = 2;
   static constexpr int kColO = 2 * kTile;               // TMEM columns: S_0, S_1, O_0, O_1
 };
 
@@ -249,101 +252,112 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------------ matrix instructions
-    // The whole warp goes through the loop, so that addresses and descriptors stay in uniform registers; one elected lane
-    // issues.
-    {
-      constexpr uint32_t kIdQk = mma_idesc<kBf16, kRows, kTile, false>();
-      constexpr uint32_t kIdPv = mma_idesc<kBf16, kRows, D, true>();
-      const uint32_t q_addr = smem_u32(smem), kv_addr = smem_u32(smem + C::kOffKv);
-      uint32_t c = 0, q_round = 0, p_par = 0;  // bit s: parity of stream s's next P
-      auto commit = [&](uint64_t *bar) {
-        if (elect_one()) tc_commit(bar);
-      };
-      for (int r = 0, item = item_of(0); item < p.items; item = item_of(++r)) {
-        const Work w = make_work(seqs, p, item);
-        if (w.n == 0) continue;
-        wait(q_full, q_round & 1);
-        ++q_round;
-        auto qk = [&](int s, uint32_t st) {
-          const uint64_t a = smem_desc(q_addr + (w.dual ? s * C::kQBytes : 0)), b = smem_desc(kv_addr + st * C::kStageBytes);
-          if (elect_one()) {
+    // This warp is the block's pace: the queue of matrix instructions is a few deep, so whatever it does between them the
+    // tensor cores wait for.  The whole warp goes through the loop (addresses and descriptors stay in uniform registers),
+    // one elected lane issues, and everything between two waits is issued in one go.
+    constexpr uint32_t kIdQk = mma_idesc<kBf16, kRows, kTile, false>();
+    constexpr uint32_t kIdPv = mma_idesc<kBf16, kRows, D, true>();
+    constexpr uint32_t kStep = C::kStageBytes >> 4;
+    const uint64_t dq = smem_desc(smem_u32(smem));
+    const uint64_t dk = smem_desc(smem_u32(smem + C::kOffKv)), dv = smem_desc(smem_u32(smem + C::kOffKv), C::kSub);
+    uint32_t st = 0, st_par = 0, q_par = 0, p_par0 = 0, p_par1 = 0;
+    auto take = [&]() {  // the next stage of the ring, filled
+      const uint32_t now = st;
+      wait(&kv_full[now], st_par);
+      if (++st == C::kStages) {
+        st = 0;
+        st_par ^= 1;
+      }
+      return now;
+    };
+    // first part of O += P V (the part's probabilities waited for), then the rest
+    auto pv = [&](int s, uint64_t b, bool acc, int k0, int k1) {
 #pragma unroll
-            for (int k = 0; k < D / 16; ++k) {
-              const uint32_t off = ((k / 4) * (kRows * 128) + (k % 4) * 32) >> 4;
-              mma_ss(tmem + s * kTile, a + off, b + off, kIdQk, k > 0);
-            }
-            tc_commit(&s_full[s]);
-          }
-        };
-        auto pv = [&](int s, uint32_t st, bool acc) {
-          const uint64_t b = smem_desc(kv_addr + st * C::kStageBytes, C::kSub);
-          wait(&p_full[s], (p_par >> s) & 1);
+      for (int k = 0; k < kTile / 16; ++k)
+        if (k >= k0 && k < k1)
+          mma_ts(tmem + C::kColO + s * D, tmem + s * kTile + k * 8, b + (k * 2048 >> 4), kIdPv, acc || k > 0);
+    };
+    auto qk = [&](int s, uint64_t a, uint64_t b) {
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) {
+        const uint32_t off = ((k / 4) * (kRows * 128) + (k % 4) * 32) >> 4;
+        mma_ss(tmem + s * kTile, a + off, b + off, kIdQk, k > 0);
+      }
+      tc_commit(&s_full[s]);
+    };
+    // waits for stream s's probabilities of a tile and issues their product up to the last part
+    auto pv_first = [&](int s, uint32_t sv, bool acc) {
+      uint32_t &par = s == 0 ? p_par0 : p_par1;
+      if (C::kPart0 < kTile) {
+        wait(&p_full[s], par);
+        tc_fence_after();
+        if (elect_one()) pv(s, dv + sv * kStep, acc, 0, C::kPart0 / 16);
+      }
+      wait(&p_rest[s], par);
+      par ^= 1;
+      tc_fence_after();
+    };
+    constexpr int kRest = C::kPart0 < kTile ? C::kPart0 / 16 : 0;  // first step that is still to be issued then
+    for (int r = 0, item = item_of(0); item < p.items; item = item_of(++r)) {
+      const Work w = make_work(seqs, p, item);
+      if (w.n == 0) continue;
+      wait(q_full, q_par);
+      q_par ^= 1;
+      if (w.dual) {
+        // V of tile j, then K of tile j + 1; the streams alternate
+        for (int j = w.it.tile0 - 1; j < w.it.tile1; ++j) {
+          const bool has_v = j >= w.it.tile0, has_k = j + 1 < w.it.tile1;
+          const uint32_t sv = has_v ? take() : 0, sk = has_k ? take() : 0;
           tc_fence_after();
-          if (elect_one())
 #pragma unroll
-            for (int k = 0; k < kPart0 / 16; ++k)
-              mma_ts(tmem + C::kColO + s * D, tmem + s * kTile + k * 8, b + (k * 2048 >> 4), kIdPv, acc || k > 0);
-          wait(&p_rest[s], (p_par >> s) & 1);
-          p_par ^= 1u << s;
-          tc_fence_after();
-          if (elect_one())
-#pragma unroll
-            for (int k = kPart0 / 16; k < kTile / 16; ++k)
-              mma_ts(tmem + C::kColO + s * D, tmem + s * kTile + k * 8, b + (k * 2048 >> 4), kIdPv, true);
-        };
-        auto take = [&]() {  // the next stage of the ring, filled
-          const uint32_t st = c % C::kStages;
-          wait(&kv_full[st], (c / C::kStages) & 1);
-          ++c;
-          tc_fence_after();
-          return st;
-        };
-        if (w.dual) {
-          for (int j = w.it.tile0 - 1; j < w.it.tile1; ++j) {
-            // V of tile j, then K of tile j + 1; the streams alternate
-            const bool has_v = j >= w.it.tile0, has_k = j + 1 < w.it.tile1;
-            const uint32_t sv = has_v ? take() : 0, sk = has_k ? take() : 0;
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-              if (has_v && j >= w.j0[s] && j < w.j1[s]) {
-                pv(s, sv, j > w.j0[s]);
-                if (j + 1 == w.j1[s]) commit(&o_full[s]);
+          for (int s = 0; s < 2; ++s) {
+            const bool av = has_v && j >= w.j0[s] && j < w.j1[s], ak = has_k && j + 1 >= w.j0[s] && j + 1 < w.j1[s];
+            if (av) pv_first(s, sv, j > w.j0[s]);
+            if (elect_one()) {
+              if (av) {
+                pv(s, dv + sv * kStep, kRest > 0 || j > w.j0[s], kRest, kTile / 16);
+                if (j + 1 == w.j1[s]) tc_commit(&o_full[s]);
               }
-              if (s == 1 && has_v) commit(&kv_empty[sv]);
-              if (has_k && j + 1 >= w.j0[s] && j + 1 < w.j1[s]) qk(s, sk);
+              if (s == 1 && has_v) tc_commit(&kv_empty[sv]);
+              if (ak) qk(s, dq + s * (C::kQBytes >> 4), dk + sk * kStep);
+              if (s == 1 && has_k) {
+                tc_commit(&kv_empty[sk]);
+                if (j + 2 >= w.it.tile1) tc_commit(q_empty);
+              }
             }
-            if (has_k) {
-              commit(&kv_empty[sk]);
-              if (j + 2 >= w.it.tile1) commit(q_empty);
-            }
+            __syncwarp();
           }
-        } else {
-          for (int i = 0; i < min(2, w.n); ++i) {
-            const uint32_t st = take();
-            qk(i, st);
-            commit(&kv_empty[st]);
-            if (i + 1 == w.n) commit(q_empty);
-          }
-          for (int i = 0; i < w.n; ++i) {
-            const int s = i & 1;
-            const uint32_t sv = take();
-            pv(s, sv, i > 1);
-            commit(&kv_empty[sv]);
-            if (i + 2 >= w.n) {
-              commit(&o_full[s]);
-              continue;
+        }
+      } else {
+        // V of tile i, then K of tile i + 2, both on stream i & 1
+        for (int i = -2; i < w.n; ++i) {
+          const bool has_v = i >= 0, has_k = i + 2 < w.n;
+          const uint32_t sv = has_v ? take() : 0, sk = has_k ? take() : 0;
+          tc_fence_after();
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            if ((i & 1) != s) continue;
+            if (has_v) pv_first(s, sv, i > 1);
+            if (elect_one()) {
+              if (has_v) {
+                pv(s, dv + sv * kStep, kRest > 0 || i > 1, kRest, kTile / 16);
+                if (i + 2 >= w.n) tc_commit(&o_full[s]);
+                tc_commit(&kv_empty[sv]);
+              }
+              if (has_k) {
+                qk(s, dq, dk + sk * kStep);
+                tc_commit(&kv_empty[sk]);
+                if (i + 3 == w.n) tc_commit(q_empty);
+              }
             }
-            const uint32_t sk = take();
-            qk(s, sk);
-            commit(&kv_empty[sk]);
-            if (i + 3 == w.n) commit(q_empty);
+            __syncwarp();
           }
         }
       }
-      commit(fin);  // every arrival that the instructions still owe has happened before the block ends
-      wait(fin, 0);
     }
+    if (elect_one()) tc_commit(fin);  // every arrival that the instructions still owe has happened before the block ends
     __syncwarp();
+    wait(fin, 0);
   } else if (warp >= 4) {
     // ------------------------------------------------------------------ softmax, one row per thread
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
@@ -429,13 +443,17 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
               const uint64_t v = fma_f32x2(pack_f32x2(__uint_as_float(x[c0 + i]), __uint_as_float(x[c0 + i + 1])), scale2, base2);
               float a, b;
               unpack_f32x2(v, a, b);
-              a = fast_exp2(a);
-              b = fast_exp2(b);
+              if ((i >> 1) % 8 < C::kPolyOf8) {
+                exp2_poly2(v, a, b);
+              } else {
+                a = fast_exp2(a);
+                b = fast_exp2(b);
+              }
               sum2[(i >> 1) & 1] = add_f32x2(sum2[(i >> 1) & 1], pack_f32x2(a, b));
               pk[i / 2] = pack2<T>(a, b);
             }
             tmem_st16(t_s + c0 / 2, pk);
-            if (c0 + 32 == kPart0) {  // the product may start on these tokens
+            if (c0 + 32 == C::kPart0 && C::kPart0 < kTile) {  // the product may start on these tokens
               tc_wait_st();
               tc_fence_before();
               __syncwarp();
@@ -446,7 +464,8 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           float s0, s1;
           unpack_f32x2(add_f32x2(sum2[0], sum2[1]), s0, s1);
           l += s0 + s1;
-        } else if (lane == 0) {
+          if (m == -INFINITY) l = 0.f;  // nothing seen so far: the polynomial's 2^-126 does not count
+        } else if (C::kPart0 < kTile && lane == 0) {
           mbar_arrive(&p_full[s]);
         }
         tc_fence_before();

@@ -128,6 +128,28 @@ __device__ __forceinline__ uint64_t mul_f32x2(uint64_t a, uint64_t b) {
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
+// 2^x of two values without the special-function unit: x = n + f with n the nearest integer (by adding and subtracting
+// 1.5 * 2^23, whose low bits then hold n) and f in [-1/2, 1/2]; 2^f by the cubic of least relative error there (7.5e-5:
+// computed for this by linear programming on a grid), n added to the exponent.  x is held above -126 (a NaN stays one), so what should
+// be 0 is 2^-126.
+__device__ __forceinline__ void exp2_poly2(uint64_t v, float &a, float &b) {
+  float x, y;
+  unpack_f32x2(v, x, y);
+  asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x));  // -126
+  asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(y));
+  v = pack_f32x2(x, y);
+  const uint64_t t = add_f32x2(v, pack_f32x2(12582912.f, 12582912.f));
+  const uint64_t f = fma_f32x2(add_f32x2(t, pack_f32x2(-12582912.f, -12582912.f)), pack_f32x2(-1.f, -1.f), v);
+  uint64_t q = fma_f32x2(f, pack_f32x2(0.05517166852951050f, 0.05517166852951050f),
+                         pack_f32x2(0.2426111251115799f, 0.2426111251115799f));
+  q = fma_f32x2(q, f, pack_f32x2(0.6932609677314758f, 0.6932609677314758f));
+  q = fma_f32x2(q, f, pack_f32x2(0.9999280571937561f, 0.9999280571937561f));
+  float tx, ty;
+  unpack_f32x2(t, tx, ty);
+  unpack_f32x2(q, x, y);
+  a = __uint_as_float(__float_as_uint(x) + (__float_as_uint(tx) << 23));
+  b = __uint_as_float(__float_as_uint(y) + (__float_as_uint(ty) << 23));
+}
 #endif  // __CUDACC__
 
 }  // namespace msco
