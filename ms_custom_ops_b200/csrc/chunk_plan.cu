@@ -165,7 +165,7 @@ int launch(const MscoChunkDesc *desc, const int32_t *q_lens, const int32_t *ctx,
     p.part_o = static_cast<float *>(workspace);
     p.part_ml = reinterpret_cast<float *>(static_cast<char *>(workspace) + part_ml_offset(d, pl));
     if (((reinterpret_cast<uintptr_t>(query) | reinterpret_cast<uintptr_t>(key_cache) |
-          reinterpret_cast<uintptr_t>(value_cache) | reinterpret_cast<uintptr_t>(out)) & 15) != 0)
+          reinterpret_cast<uintptr_t>(value_cache)) & 15) != 0 || (reinterpret_cast<uintptr_t>(out) & 31) != 0)
       tc = false;  // rows that the copies cannot start on: the general kernel takes them
   }
   const int sms = tc ? sm_count() : 0;

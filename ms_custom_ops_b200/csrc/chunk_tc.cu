@@ -6,13 +6,13 @@
 //   rows > 128   ("dual")   stream s owns rows 128 s .. 128 s + 127, both go over all KV tiles
 //   rows <= 128  ("single") both streams own the same rows, stream s the KV tiles s, s + 2, ...; their states
 //                           are merged at the end
-// Per tile and stream:  S = Q K^T (shared x shared -> TMEM),  P = 2^(S scale - m) (registers, one row per thread, back
+// Per tile and stream:  S = Q K^T (shared x shared -> TMEM),  P = 2^(S scale - m) (registers, half a row per thread, back
 // to TMEM in 16 bits over S),  O += P V (TMEM x shared -> TMEM).  The running maximum only moves when it grows by
 // more than kSlack (a factor 256): until then P is up to 256 instead of 1, which costs no precision in a floating
 // format, and O stays where it is; it is rescaled in TMEM by the softmax warps in the rare tiles where it must.
 //
 // Warps: 0 loads (TMA, 128-byte swizzle), 1 matrix instructions (2, 3 idle: registers are handed out by groups of four
-// warps), 4-7 / 8-11 softmax of stream 0 / 1.
+// warps), 4-11 / 12-19 softmax of stream 0 / 1.
 // The matrix instructions are issued O_0 += P_0 V, S_0 = Q_0 K', O_1 += P_1 V, S_1 = Q_1 K' (K' the next tile); they execute in
 // that order, so a completed S' means that the product that read P, which lies over it, is complete too.
 #include <cuda.h>
@@ -29,7 +29,8 @@ namespace {
 
 constexpr int kRows = 128;        // rows of one stream
 constexpr int kTile = kChunkKvTile;
-constexpr int kThreads = 384;
+constexpr int kThreads = 640;
+constexpr int kSoftWarps = 8;     // per stream
 constexpr float kSlack = 8.f;     // log2 of how far a probability may exceed 1
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr uint32_t kWaitLimit = 1u << 22;
@@ -44,14 +45,13 @@ struct Cfg {
   static constexpr int kStageBytes = kTile * D * 2;
   static constexpr int kQBytes = kRows * D * 2;
   static constexpr int kStages = D == 128 ? 5 : 10;
-  // tokens of a tile whose probabilities are handed over first (kTile: all at once)
-  static constexpr int kPart0 = D == 128 ? 96 : kTile;
+  // tokens of each half of a tile whose probabilities are handed over first (64: all at once)
+  static constexpr int kPart0 = D == 128 ? 32 : 64;
   static constexpr int kOffKv = 2 * kQBytes;
   static constexpr int kOffBar = kOffKv + kStages * kStageBytes;
   static constexpr int kNumBars = 2 * kStages + 12;
-  static constexpr int kOffMl = kOffBar + kNumBars * 8 + 16;  // [128][2] floats of the merge of the streams
-  static constexpr int kSmem = kOffMl + kRows * 2 * 4;
-  static constexpr int kDynSmem = kSmem + 1024;
+  static constexpr int kOffXch = kOffBar + kNumBars * 8 + 16;  // [stream][half][row]: what the two threads of a row exchange
+  static constexpr int kSmem = kOffXch + 2 * 2 * kRows * 4;
   // of eight pairs of probabilities, those that are computed by the FMA pipe
   static constexpr int kPolyOf8 = 2;
   static constexpr int kColO = 2 * kTile;               // TMEM columns: S_0, S_1, O_0, O_1
@@ -84,6 +84,13 @@ struct Work {
   int j0[2], j1[2];  // tiles of each stream, absolute
   int step;     // 1 (dual) or 2
 };
+
+// 32 aligned bytes: a whole sector in one store
+__device__ __forceinline__ void store_32b(void *p, const uint32_t *r) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
+               "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
 
 template <int N>
 __device__ __forceinline__ Work make_work(const ChunkSeqs<N> &seqs, const ChunkParams &p, int item) {
@@ -126,8 +133,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
                 const __grid_constant__ ChunkSeqs<N> seqs) {
   using C = Cfg<D>;
   constexpr bool kBf16 = sizeof(T) == 2 && !std::is_same<T, __half>::value;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t *bars = reinterpret_cast<uint64_t *>(smem + C::kOffBar);
   uint64_t *kv_full = bars, *kv_empty = bars + C::kStages;
   uint64_t *q_full = bars + 2 * C::kStages, *q_empty = q_full + 1, *s_full = q_full + 2, *p_full = q_full + 4,
@@ -135,7 +141,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
            *p_rest = q_full + 10;
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + C::kNumBars);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
-  float *ml = reinterpret_cast<float *>(smem + C::kOffMl);
+  float *xch = reinterpret_cast<float *>(smem + C::kOffXch);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (threadIdx.x == 0) {
@@ -147,8 +153,8 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     mbar_init(q_empty, 2);
     for (int s = 0; s < 2; ++s) {
       mbar_init(&s_full[s], 1);
-      mbar_init(&p_full[s], 4);
-      mbar_init(&p_rest[s], 4);
+      mbar_init(&p_full[s], kSoftWarps);
+      mbar_init(&p_rest[s], kSoftWarps);
       mbar_init(&o_full[s], 1);
     }
     mbar_init(tail, 1);
@@ -164,8 +170,8 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   const Waiter wait{abort_flag};
   const int half = p.item_tokens >> 1;
 
-  // Registers: 384 x 168 at launch = 256 x 208 (softmax) + 128 x 88 (the first four warps)
-  if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+  // Registers: 640 x 96 at launch = 512 x 104 (softmax) + 128 x 64 (the first four warps)
+  if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
   if (warp == 0) {
     // ------------------------------------------------------------------ loads
     if (lane == 0) {
@@ -270,12 +276,13 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       }
       return now;
     };
-    // first part of O += P V (the part's probabilities waited for), then the rest
-    auto pv = [&](int s, uint64_t b, bool acc, int k0, int k1) {
+    // O += P V over the first (part 0) or the other tokens of each half of the tile; the halves' P lie 64 columns apart
+    auto pv = [&](int s, uint64_t b, bool acc, int part) {
 #pragma unroll
       for (int k = 0; k < kTile / 16; ++k)
-        if (k >= k0 && k < k1)
-          mma_ts(tmem + C::kColO + s * D, tmem + s * kTile + k * 8, b + (k * 2048 >> 4), kIdPv, acc || k > 0);
+        if (((k & 3) * 16 < C::kPart0) == (part == 0))
+          mma_ts(tmem + C::kColO + s * D, tmem + s * kTile + (k >> 2) * 64 + (k & 3) * 8, b + (k * 2048 >> 4), kIdPv,
+                 acc || k > 0);
     };
     auto qk = [&](int s, uint64_t a, uint64_t b) {
 #pragma unroll
@@ -286,18 +293,18 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       tc_commit(&s_full[s]);
     };
     // waits for stream s's probabilities of a tile and issues their product up to the last part
+    constexpr bool kParts = C::kPart0 < 64;
     auto pv_first = [&](int s, uint32_t sv, bool acc) {
       uint32_t &par = s == 0 ? p_par0 : p_par1;
-      if (C::kPart0 < kTile) {
+      if (kParts) {
         wait(&p_full[s], par);
         tc_fence_after();
-        if (elect_one()) pv(s, dv + sv * kStep, acc, 0, C::kPart0 / 16);
+        if (elect_one()) pv(s, dv + sv * kStep, acc, 0);
       }
       wait(&p_rest[s], par);
       par ^= 1;
       tc_fence_after();
     };
-    constexpr int kRest = C::kPart0 < kTile ? C::kPart0 / 16 : 0;  // first step that is still to be issued then
     for (int r = 0, item = item_of(0); item < p.items; item = item_of(++r)) {
       const Work w = make_work(seqs, p, item);
       if (w.n == 0) continue;
@@ -315,7 +322,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
             if (av) pv_first(s, sv, j > w.j0[s]);
             if (elect_one()) {
               if (av) {
-                pv(s, dv + sv * kStep, kRest > 0 || j > w.j0[s], kRest, kTile / 16);
+                pv(s, dv + sv * kStep, kParts || j > w.j0[s], kParts ? 1 : 0);
                 if (j + 1 == w.j1[s]) tc_commit(&o_full[s]);
               }
               if (s == 1 && has_v) tc_commit(&kv_empty[sv]);
@@ -340,7 +347,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
             if (has_v) pv_first(s, sv, i > 1);
             if (elect_one()) {
               if (has_v) {
-                pv(s, dv + sv * kStep, kRest > 0 || i > 1, kRest, kTile / 16);
+                pv(s, dv + sv * kStep, kParts || i > 1, kParts ? 1 : 0);
                 if (i + 2 >= w.n) tc_commit(&o_full[s]);
                 tc_commit(&kv_empty[sv]);
               }
@@ -359,14 +366,19 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     __syncwarp();
     wait(fin, 0);
   } else if (warp >= 4) {
-    // ------------------------------------------------------------------ softmax, one row per thread
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-    const int s = (warp >> 2) - 1;
-    const int row = threadIdx.x & 127;
+    // ------------------------------------------------------------------ softmax, two threads per row
+    // The threads of a row are in two warps, one for each half of a tile's columns (and of O's): with four softmax warps
+    // on each scheduler the latencies of one hide behind the others.  They exchange their halves' maxima.
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+    const int s = (warp - 4) >> 3, hf = ((warp >> 2) & 1) ^ 1;
+    const int row = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)(warp & 3) * 32 << 16;
-    const uint32_t t_s = tmem + lanes + s * kTile, t_o = tmem + lanes + C::kColO + s * D;
+    const uint32_t t_s = tmem + lanes + s * kTile + hf * 64, t_o = tmem + lanes + C::kColO + s * D + hf * (D / 2);
+    const int pair = 1 + s * 4 + (warp & 3);  // named barrier of the two warps of these rows
+    float *x_mine = xch + (s * 2 + hf) * kRows + row, *x_other = xch + (s * 2 + (hf ^ 1)) * kRows + row;
     const int g = p.group;
     const int tok_in = row / g, head_in = row - tok_in * g;
+    const bool speaker = s == 1 && hf == 0 && (warp & 3) == 0;  // the warp that frees Q's space for its stream
     uint32_t s_round = 0, o_round = 0, q_round = 0;
     for (int r = 0, item = item_of(0); item < p.items; item = item_of(++r)) {
       const Work w = make_work(seqs, p, item);
@@ -379,7 +391,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       const int pos = live ? pos0 + tok_in : -1;
       const int j_beg = s == 0 ? w.j0[0] : w.j0[1], j_end = s == 0 ? w.j1[0] : w.j1[1];
       float m = -INFINITY, l = 0.f;
-      if (warp == 8 && w.n > 0) {
+      if (speaker && w.n > 0) {
         // One of the two arrivals that free Q's space is stream 1's: at once (dual), or when the merge is through with it
         // (single).  It comes behind the arrival of the item's rows, so never before the one of the item in front.
         wait(q_full, q_round & 1);
@@ -391,29 +403,34 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         ++s_round;
         tc_fence_after();
         if (warp_live) {
-          uint32_t x[kTile];
+          uint32_t x[64];
+          tmem_ld32(t_s, x);
+          tmem_ld32(t_s + 32, x + 32);
+          tmem_wait_ld32(x);
+          tmem_wait_ld32(x + 32);
+          const int col0 = j * kTile + hf * 64;
+          if (pos0 < col0 + 63 || (p.window > 0 && pos0 + ntok - p.window > col0)) {
+            const int hi = pos - col0;                                    // columns 0 .. hi are seen
+            const int lo = p.window > 0 ? pos - p.window + 1 - col0 : 0;  // from column lo on
 #pragma unroll
-          for (int c = 0; c < kTile; c += 32) tmem_ld32(t_s + c, x + c);
-#pragma unroll
-          for (int c = 0; c < kTile; c += 32) tmem_wait_ld32(x + c);
-          const int hi = pos - j * kTile;                                     // columns 0 .. hi are seen
-          const int lo = p.window > 0 ? pos - p.window + 1 - j * kTile : 0;   // from column lo on
-          if (pos0 < (j + 1) * kTile - 1 || (p.window > 0 && pos0 + ntok - p.window > j * kTile)) {
-#pragma unroll
-            for (int c = 0; c < kTile; ++c) x[c] = c <= hi && c >= lo ? x[c] : 0xff800000u;  // -inf
+            for (int c = 0; c < 64; ++c) x[c] = c <= hi && c >= lo ? x[c] : 0xff800000u;  // -inf
           }
-          // four chains of three-way maxima: one chain would be 128 dependent steps
+          // four chains of three-way maxima: one chain would be 64 dependent steps
           float mx4[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) mx4[i] = __uint_as_float(x[i]);
 #pragma unroll
-          for (int c = 4; c < kTile - 4; c += 8)
+          for (int c = 4; c < 60; c += 8)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
               mx4[i] = fmaxf(mx4[i], fmaxf(__uint_as_float(x[c + i]), __uint_as_float(x[c + 4 + i])));
 #pragma unroll
-          for (int i = 0; i < 4; ++i) mx4[i] = fmaxf(mx4[i], __uint_as_float(x[kTile - 4 + i]));
-          const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * p.scale_log2e;
+          for (int i = 0; i < 4; ++i) mx4[i] = fmaxf(mx4[i], __uint_as_float(x[60 + i]));
+          float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+          // (the next tile's exchange comes behind that tile's s_full, which both warps' p_rest of this one precede)
+          *x_mine = mx;
+          named_bar_sync(pair, 64);
+          mx = fmaxf(mx, *x_other) * p.scale_log2e;
           const bool first = j == j_beg;
           const bool grow = mx > m + kSlack;  // also for the first value: m is -inf
           if (__any_sync(0xffffffffu, grow)) {
@@ -421,14 +438,14 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
             m = grow ? mx : m;
             l *= w_old;
             if (!first) {
+#pragma unroll 1
+              for (int c = 0; c < D / 2; c += 16) {
+                uint32_t o[16];
+                tmem_ld16(t_o + c, o);
+                tmem_wait_ld16(o);
 #pragma unroll
-              for (int c = 0; c < D; c += 32) {
-                uint32_t o[32];
-                tmem_ld32(t_o + c, o);
-                tmem_wait_ld32(o);
-#pragma unroll
-                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * w_old);
-                tmem_st32(t_o + c, o);
+                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * w_old);
+                tmem_st16(t_o + c, o);
               }
             }
           }
@@ -436,7 +453,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           const uint64_t scale2 = pack_f32x2(p.scale_log2e, p.scale_log2e), base2 = pack_f32x2(-base, -base);
           uint64_t sum2[2] = {0, 0};
 #pragma unroll
-          for (int c0 = 0; c0 < kTile; c0 += 32) {
+          for (int c0 = 0; c0 < 64; c0 += 32) {
             uint32_t pk[16];
 #pragma unroll
             for (int i = 0; i < 32; i += 2) {
@@ -453,7 +470,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
               pk[i / 2] = pack2<T>(a, b);
             }
             tmem_st16(t_s + c0 / 2, pk);
-            if (c0 + 32 == C::kPart0 && C::kPart0 < kTile) {  // the product may start on these tokens
+            if (c0 + 32 == C::kPart0 && C::kPart0 < 64) {  // the product may start on these tokens
               tc_wait_st();
               tc_fence_before();
               __syncwarp();
@@ -461,16 +478,17 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
             }
           }
           tc_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_rest[s]);
           float s0, s1;
           unpack_f32x2(add_f32x2(sum2[0], sum2[1]), s0, s1);
           l += s0 + s1;
           if (m == -INFINITY) l = 0.f;  // nothing seen so far: the polynomial's 2^-126 does not count
-        } else if (C::kPart0 < kTile && lane == 0) {
-          mbar_arrive(&p_full[s]);
+        } else if (lane == 0) {
+          if (C::kPart0 < 64) mbar_arrive(&p_full[s]);
+          mbar_arrive(&p_rest[s]);
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_rest[s]);
       }
       // ---- the item's result
       const bool has = j_beg < j_end;
@@ -479,20 +497,27 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         ++o_round;
         tc_fence_after();
       }
-      const bool two = !w.dual && w.n > 1;  // two states of the same rows
-      float scale = 1.f, m_out = m, l_out = l;
-      if (two && s == 1) {
-        ml[row * 2] = m;
-        ml[row * 2 + 1] = l;
+      // the row's sum (o_full: both warps are through with the exchanges of the tiles)
+      if (warp_live) {
+        *x_mine = l;
+        named_bar_sync(pair, 64);
+        l += *x_other;
       }
+      const bool two = !w.dual && w.n > 1;  // two states of the same rows
+      float scale0 = 1.f, scale1 = 0.f, m_out = m, l_out = l;
       if (two) {
-        named_bar_sync(1, 256);
+        if (s == 1) {
+          if (warp_live) named_bar_sync(pair, 64);  // the sums have been read
+          *x_mine = hf == 0 ? m : l;
+        }
+        named_bar_sync(9, 512);
         if (s == 0) {
-          const float m1 = ml[row * 2], l1 = ml[row * 2 + 1];
+          const float m1 = xch[2 * kRows + row], l1 = xch[3 * kRows + row];
           m_out = fmaxf(m, m1);
           const float b = m_out == -INFINITY ? 0.f : m_out;
-          scale = fast_exp2(m - b);
-          l_out = l * scale + l1 * fast_exp2(m1 - b);
+          scale0 = fast_exp2(m - b);
+          scale1 = fast_exp2(m1 - b);
+          l_out = l * scale0 + l1 * scale1;
         }
       }
       const int64_t tok = (int64_t)e.q_start + tok0 + tok_in;
@@ -504,73 +529,60 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
                            (tok0 - w.it.tok0) * g + row;
       const float inv = split ? 1.f : (l_out > 0.f ? 1.f / l_out : 0.f);
       const bool writes = live && (w.dual || s == 0);
-      constexpr int kPart = D / 2;  // columns that go through the merge buffer at a time (the space of Q's second tile)
-      float *buf = reinterpret_cast<float *>(smem + C::kQBytes);
+      constexpr int kPart = D / 4;  // this half's columns that go through the merge buffer (the space of Q's second tile) at a time
+      float *buf = reinterpret_cast<float *>(smem + C::kQBytes) + hf * (kPart * kRows) + row;
 #pragma unroll 1
-      for (int c0 = 0; c0 < D; c0 += kPart) {
-        if (two && s == 1) {
-          // stream 1's columns of this part, column by column (consecutive rows: no bank conflicts); stream 0 weights
-          if (warp_live) {
+      for (int c0 = 0; c0 < D / 2; c0 += kPart) {
+#pragma unroll 1
+        for (int c = 0; c < kPart; c += 16) {
+          uint32_t o[16];
+          if (warp_live && has) {
+            tmem_ld16(t_o + c0 + c, o);
+            tmem_wait_ld16(o);
+          } else {
 #pragma unroll
-            for (int c = 0; c < kPart; c += 32) {
-              uint32_t o[32];
-              tmem_ld32(t_o + c0 + c, o);
-              tmem_wait_ld32(o);
-#pragma unroll
-              for (int i = 0; i < 32; ++i) buf[(c + i) * kRows + row] = __uint_as_float(o[i]);
-            }
+            for (int i = 0; i < 16; ++i) o[i] = 0;
           }
-          named_bar_sync(1, 256);
-          fence_proxy_async();  // the buffer's next use is by the loads
-          named_bar_sync(2, 256);
-          continue;
-        }
-        if (two) named_bar_sync(1, 256);
-        if (warp_live && (w.dual || s == 0)) {
-          const float s1 = two ? fast_exp2(ml[row * 2] - (m_out == -INFINITY ? 0.f : m_out)) : 0.f;
+          if (two) {
+            // stream 1 lays its columns down one by one (consecutive rows: no bank conflicts), stream 0 adds them in
+            if (s == 1) {
 #pragma unroll
-          for (int c = 0; c < kPart; c += 32) {
-            uint32_t o[32];
-            if (has) {
-              tmem_ld32(t_o + c0 + c, o);
-              tmem_wait_ld32(o);
+              for (int i = 0; i < 16; ++i) buf[(c + i) * kRows] = __uint_as_float(o[i]);
+              if (c + 16 < kPart) continue;
+            }
+            if (c == (s == 1 ? kPart - 16 : 0)) named_bar_sync(9, 512);
+            if (s == 1) continue;
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              o[i] = __float_as_uint(__uint_as_float(o[i]) * scale0 + buf[(c + i) * kRows] * scale1);
+          }
+          if (writes) {
+            const int col = hf * (D / 2) + c0 + c;
+            if (split) {
+              float *dst = p.part_o + prow * D + col;
+              store_32b(dst, o);
+              store_32b(dst + 8, o + 8);
             } else {
+              uint32_t pk[8];
 #pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = 0;
-            }
-            float f[32];
-#pragma unroll
-            for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(o[i]);
-            if (two) {
-#pragma unroll
-              for (int i = 0; i < 32; ++i) f[i] = f[i] * scale + buf[(c + i) * kRows + row] * s1;
-            }
-            if (writes) {
-              if (split) {
-                float4 *dst = reinterpret_cast<float4 *>(p.part_o + prow * D + c0 + c);
-#pragma unroll
-                for (int i = 0; i < 32; i += 4) dst[i / 4] = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
-              } else {
-                uint4 *dst = reinterpret_cast<uint4 *>(static_cast<T *>(p.out) + orow * D + c0 + c);
-#pragma unroll
-                for (int i = 0; i < 32; i += 8)
-                  dst[i / 8] = make_uint4(pack2<T>(f[i] * inv, f[i + 1] * inv), pack2<T>(f[i + 2] * inv, f[i + 3] * inv),
-                                          pack2<T>(f[i + 4] * inv, f[i + 5] * inv), pack2<T>(f[i + 6] * inv, f[i + 7] * inv));
-              }
+              for (int i = 0; i < 8; ++i) pk[i] = pack2<T>(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
+              store_32b(static_cast<T *>(p.out) + orow * D + col, pk);
             }
           }
         }
         if (two) {
-          fence_proxy_async();
-          named_bar_sync(2, 256);
+          fence_proxy_async();  // the buffer's next use is by the loads
+          named_bar_sync(10, 512);
         }
       }
       // the merge buffer lies over Q's second tile: only now may the next item's rows come in
-      if (warp == 8 && w.n > 0 && !w.dual && lane == 0) mbar_arrive(q_empty);
-      if (writes) {
+      if (speaker && w.n > 0 && !w.dual && lane == 0) mbar_arrive(q_empty);
+      if (writes && hf == 0) {
         if (split) *reinterpret_cast<float2 *>(p.part_ml + prow * 2) = make_float2(m_out, l_out);
         else if (p.lse != nullptr) p.lse[orow] = l_out > 0.f ? (m_out + log2f(l_out)) * kLn2 : -INFINITY;
       }
+      // the sums have been read before the next item's exchanges
+      if (warp_live && !two) named_bar_sync(pair, 64);
       tc_fence_before();  // the reads of O are ordered before the next item's products (which wait for its P)
     }
   }
@@ -662,7 +674,7 @@ template <typename T, int D, int N>
 int launch_sized(const MscoChunkDesc &d, const ChunkParams &p, const ChunkSeq *src, int64_t q_rows, int sms,
                  cudaStream_t stream) {
   using C = Cfg<D>;
-  static_assert(C::kDynSmem <= 232448, "shared memory of one SM exceeded");
+  static_assert(C::kSmem <= 232448, "shared memory of one SM exceeded");
   const cuuint64_t h = (cuuint64_t)d.num_kv_heads, bs = (cuuint64_t)d.block_size, nb = (cuuint64_t)d.num_blocks;
   const cuuint32_t rows = (cuuint32_t)std::min(d.block_size, kTile);
   CUtensorMap tq, tk, tv;
@@ -690,8 +702,8 @@ int launch_sized(const MscoChunkDesc &d, const ChunkParams &p, const ChunkSeq *s
   }
   auto kfn = chunk_tc_kernel<T, D, N>;
   // set per call: the attribute belongs to a device
-  MSCO_CUDA_CHECK(cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kDynSmem));
-  kfn<<<std::min(p.items, sms), kThreads, C::kDynSmem, stream>>>(tq, tk, tv, p, seqs);
+  MSCO_CUDA_CHECK(cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+  kfn<<<std::min(p.items, sms), kThreads, C::kSmem, stream>>>(tq, tk, tv, p, seqs);
   MSCO_CUDA_CHECK(cudaGetLastError());
   if (split) {
     cudaLaunchConfig_t cfg = {};

@@ -75,6 +75,12 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t *r) {
         MSCO_R4(r, 28)
       : "r"(addr));
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t *r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : MSCO_R4(r, 0), MSCO_R4(r, 4), MSCO_R4(r, 8), MSCO_R4(r, 12)
+      : "r"(addr));
+}
 __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t *r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
@@ -97,6 +103,12 @@ __device__ __forceinline__ void tmem_wait_ld32(uint32_t *r) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
                : MSCO_T4(r, 0), MSCO_T4(r, 4), MSCO_T4(r, 8), MSCO_T4(r, 12), MSCO_T4(r, 16), MSCO_T4(r, 20), MSCO_T4(r, 24),
                  MSCO_T4(r, 28)
+               :
+               : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld16(uint32_t *r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : MSCO_T4(r, 0), MSCO_T4(r, 4), MSCO_T4(r, 8), MSCO_T4(r, 12)
                :
                : "memory");
 }
