@@ -1,4 +1,4 @@
-// Chunk attention on the 5th-generation tensor cores: head_dim 64 / 128, 16-bit caches.
+// Chunk attention on the 5th-generation tensor cores: head_dim 64 / 128, 16-bit and int8 caches.
 //
 // An item is up to 256 packed rows of one kv head (token-major, the q heads of the group adjacent) against the
 // cached tokens that they see, or a split of them, 128 at a time.  Two streams keep the tensor cores busy:
@@ -11,14 +11,15 @@
 // more than kSlack (a factor 256): until then P is up to 256 instead of 1, which costs no precision in a floating
 // format, and O stays where it is; it is rescaled in TMEM by the softmax warps in the rare tiles where it must.
 //
-// Warps: 0 loads (TMA, 128-byte swizzle), 1 matrix instructions (2, 3 idle: registers are handed out by groups of four
-// warps), 4-11 / 12-19 softmax of stream 0 / 1.
+// Warps: 0 loads (TMA, 128-byte swizzle), 1 matrix instructions, 2 / 3 int8 to fp16 (16-bit caches: idle; registers are
+// handed out by groups of four warps), 4-11 / 12-19 softmax of stream 0 / 1.
 // The matrix instructions are issued O_0 += P_0 V, S_0 = Q_0 K', O_1 += P_1 V, S_1 = Q_1 K' (K' the next tile); they execute in
 // that order, so a completed S' means that the product that read P, which lies over it, is complete too.
 #include <cuda.h>
 
 #include <algorithm>
 #include <mutex>
+#include <type_traits>
 
 #include "chunk_params.h"
 #include "msco_common.cuh"
@@ -37,33 +38,47 @@ constexpr uint32_t kWaitLimit = 1u << 22;
 
 __device__ int g_chunk_error;  // MSCO_ERR_TIMEOUT once a bounded wait has run out
 
-template <int D>
+template <int D, bool KV8>
 struct Cfg {
   static_assert(D == 64 || D == 128, "head_dim 64 or 128");
   static constexpr int kBoxes = D / 64;                 // 128-byte wide sub-tiles of a row
   static constexpr int kSub = kTile * 128;              // bytes of one sub-tile
   static constexpr int kStageBytes = kTile * D * 2;
   static constexpr int kQBytes = kRows * D * 2;
-  static constexpr int kStages = D == 128 ? 5 : 10;
-  // tokens of each half of a tile whose probabilities are handed over first (64: all at once)
-  static constexpr int kPart0 = D == 128 ? 32 : 64;
+  // ring of 16-bit tiles; int8 caches: four of them (what the matrix instructions look ahead) behind a ring of raw tiles
+  static constexpr int kStages = KV8 ? 4 : (D == 128 ? 5 : 10);
+  static constexpr int kRawBytes = kTile * D;
+  static constexpr int kRaw = KV8 ? (D == 128 ? 2 : 8) : 0;
   static constexpr int kOffKv = 2 * kQBytes;
-  static constexpr int kOffBar = kOffKv + kStages * kStageBytes;
-  static constexpr int kNumBars = 2 * kStages + 12;
+  static constexpr int kOffRaw = kOffKv + kStages * kStageBytes;
+  static constexpr int kOffBar = kOffRaw + kRaw * kRawBytes;
+  static constexpr int kNumBars = 2 * kStages + 2 * kRaw + 10;
   static constexpr int kOffXch = kOffBar + kNumBars * 8 + 16;  // [stream][half][row]: what the two threads of a row exchange
-  static constexpr int kSmem = kOffXch + 2 * 2 * kRows * 4;
-  // of eight pairs of probabilities, those that are computed by the FMA pipe
-  static constexpr int kPolyOf8 = 2;
+  static constexpr int kSmem = kOffXch + 2 * 2 * kRows * 4 + (KV8 ? kRows * 4 : 0);
+  // Of eight pairs of probabilities, those whose exponentials the FMA pipe computes.  At head_dim 128 the special-function
+  // unit alone (1024 clocks a tile and stream) is as long as the two products: 2 of 8 took the prompt of 8192 tokens from
+  // 503 to 460 us, 3 of 8 gave 475; at 64, where issue slots are short, any made it slower (316 us without, 355 with 2).
+  static constexpr int kPolyOf8 = D == 128 ? 2 : 0;
   static constexpr int kColO = 2 * kTile;               // TMEM columns: S_0, S_1, O_0, O_1
 };
 
 // A bounded wait on an mbarrier.  Should one run out (a lost arrival), the block's flag is set, every wait of the block
 // returns at once from then on, and all roles run through the rest of their loops without waiting: whatever they do
 // stays inside their buffers, the result is worthless and the device's error word says so.
+__device__ __forceinline__ bool mbar_try_wait_at(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
 struct Waiter {
   volatile int *abort;
-  __device__ __forceinline__ void operator()(uint64_t *bar, uint32_t parity) const {  // by a whole warp
-    for (uint32_t i = 0; !mbar_try_wait(bar, parity); ++i) {
+  __device__ __forceinline__ void operator()(uint64_t *bar, uint32_t parity) const { (*this)(smem_u32(bar), parity); }
+  __device__ __forceinline__ void operator()(uint32_t bar, uint32_t parity) const {  // by a whole warp
+    for (uint32_t i = 0; !mbar_try_wait_at(bar, parity); ++i) {
       if ((i & 255) != 255) continue;
       if (*abort) break;
       if (i >= kWaitLimit) {
@@ -84,6 +99,12 @@ struct Work {
   int j0[2], j1[2];  // tiles of each stream, absolute
   int step;     // 1 (dual) or 2
 };
+
+// int8 cache: value of channel `c` from the mean x of its raw values (inv 0: nothing seen, stays 0)
+__device__ __forceinline__ float dequant_out(const ChunkParams &p, int c, float x, float inv) {
+  if (p.v_offset != nullptr && inv != 0.f) x += (float)__ldg(p.v_offset + c);
+  return x * __ldg(p.v_descale + c);
+}
 
 // 32 aligned bytes: a whole sector in one store
 __device__ __forceinline__ void store_32b(void *p, const uint32_t *r) {
@@ -126,35 +147,40 @@ __device__ __forceinline__ int item_of(int r) {
   return r * g + ((r & 1) ? g - 1 - c : c);
 }
 
-template <typename T, int D, int N>
+template <typename T, int D, bool KV8, int N>
 __global__ void __launch_bounds__(kThreads, 1)
 chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                 const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ ChunkParams p,
                 const __grid_constant__ ChunkSeqs<N> seqs) {
-  using C = Cfg<D>;
-  constexpr bool kBf16 = sizeof(T) == 2 && !std::is_same<T, __half>::value;
+  using C = Cfg<D, KV8>;
+  // int8 caches: all operands fp16, in which every int8 is exact
+  using M = typename std::conditional<KV8, __half, T>::type;
+  constexpr bool kBf16 = !std::is_same<M, __half>::value;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t *bars = reinterpret_cast<uint64_t *>(smem + C::kOffBar);
   uint64_t *kv_full = bars, *kv_empty = bars + C::kStages;
   uint64_t *q_full = bars + 2 * C::kStages, *q_empty = q_full + 1, *s_full = q_full + 2, *p_full = q_full + 4,
-           *o_full = q_full + 6, *tail = q_full + 8, *fin = q_full + 9,
-           *p_rest = q_full + 10;
+           *o_full = q_full + 6, *tail = q_full + 8, *fin = q_full + 9, *raw_full = q_full + 10, *raw_empty = raw_full + C::kRaw;
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + C::kNumBars);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
   float *xch = reinterpret_cast<float *>(smem + C::kOffXch);
+  float *q_scale = xch + 2 * 2 * kRows;  // int8, single: what stream 0 found for the rows
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (threadIdx.x == 0) {
     for (int i = 0; i < C::kStages; ++i) {
-      mbar_init(&kv_full[i], 1);
+      mbar_init(&kv_full[i], KV8 ? 2 : 1);  // the copy, or the two converting warps
       mbar_init(&kv_empty[i], 1);
     }
-    mbar_init(q_full, 1);
+    mbar_init(q_full, KV8 ? 2 * kSoftWarps : 1);
+    for (int i = 0; i < C::kRaw; ++i) {
+      mbar_init(&raw_full[i], 1);
+      mbar_init(&raw_empty[i], 2);
+    }
     mbar_init(q_empty, 2);
     for (int s = 0; s < 2; ++s) {
       mbar_init(&s_full[s], 1);
       mbar_init(&p_full[s], kSoftWarps);
-      mbar_init(&p_rest[s], kSoftWarps);
       mbar_init(&o_full[s], 1);
     }
     mbar_init(tail, 1);
@@ -189,9 +215,9 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       // cached tokens that some new token of the sequence sees: the rest of the table may hold anything
       const int alive0 = p.window > 0 ? max(0, e.ctx - e.q_len - p.window + 1) : 0, alive1 = e.ctx;
       const int32_t *table = p.block_tables + (int64_t)e.row * p.max_blocks_per_seq;
-      if (q_round > 0) wait(q_empty, (q_round - 1) & 1);
+      if (!KV8 && q_round > 0) wait(q_empty, (q_round - 1) & 1);
       ++q_round;
-      if (lane == 0) {
+      if (!KV8 && lane == 0) {  // (int8: the softmax warps fold the scales into the query rows)
         const int tiles = w.dual ? 2 : 1;
         mbar_arrive_expect_tx(q_full, (uint32_t)(tiles * C::kBoxes * half * p.group * 128));
         for (int s = 0; s < tiles; ++s)
@@ -203,16 +229,18 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       int32_t id = 0;
       // one tile of K or V into the next stage of the ring
       auto load = [&](const CUtensorMap *tm, int j, bool is_v) {
-        const uint32_t st = c % C::kStages, use = c / C::kStages;
+        constexpr int kRing = KV8 ? C::kRaw : C::kStages;
+        const uint32_t st = c % kRing, use = c / kRing;
         ++c;
-        if (use > 0) wait(&kv_empty[st], (use - 1) & 1);
-        uint8_t *dst = smem + C::kOffKv + st * C::kStageBytes;
+        if (use > 0) wait(KV8 ? &raw_empty[st] : &kv_empty[st], (use - 1) & 1);
+        uint8_t *dst = smem + (KV8 ? C::kOffRaw + st * C::kRawBytes : C::kOffKv + st * C::kStageBytes);
         const int tok = j * kTile;
         const int a = max(0, alive0 - tok), b = min(kTile, alive1 - tok);  // rows of the tile that are alive
         const int b0 = a / box_rows, b1 = (b + box_rows - 1) / box_rows;   // boxes that hold some of them
         // a V row that is not alive is zeroed: its probability is 0, but what it holds may not be finite
-        const bool patch = is_v && (a > 0 || b < kTile);
-        uint64_t *bar = patch ? tail : &kv_full[st];
+        // (int8: the converting warps see to it)
+        const bool patch = !KV8 && is_v && (a > 0 || b < kTile);
+        uint64_t *bar = KV8 ? &raw_full[st] : (patch ? tail : &kv_full[st]);
         const int col = (tok + lane * box_rows) / bs;  // this lane's block-table column (boxes <= 16)
         const int first = tok / bs;
         if (win < 0 || first < win || (tok + kTile - 1) / bs >= win + 32) {
@@ -222,7 +250,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         }
         const bool mine = lane >= b0 && lane < b1 && lane < boxes;
         int32_t blk = __shfl_sync(0xffffffffu, id, mine ? col - win : 0);
-        if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)((b1 - b0) * box_rows * 128 * C::kBoxes));
+        if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)((b1 - b0) * box_rows * (KV8 ? D : 2 * D)));
         __syncwarp();
         if (mine) {
           if (blk < 0 || blk >= p.num_blocks) {
@@ -232,8 +260,12 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           const int off = (tok + lane * box_rows) % bs;
           const int y = p.cache_layout == 1 ? off : w.it.kvh;
           const int z = p.cache_layout == 1 ? blk * p.num_kv_heads + w.it.kvh : blk * bs + off;
+          if (KV8) {
+            tma_load_3d(dst + lane * box_rows * D, tm, 0, y, z, bar);
+          } else {
 #pragma unroll
-          for (int x = 0; x < C::kBoxes; ++x) tma_load_3d(dst + x * C::kSub + lane * box_rows * 128, tm, x * 64, y, z, bar);
+            for (int x = 0; x < C::kBoxes; ++x) tma_load_3d(dst + x * C::kSub + lane * box_rows * 128, tm, x * 64, y, z, bar);
+          }
         }
         if (patch) {
           wait(tail, tails & 1);
@@ -266,23 +298,22 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     constexpr uint32_t kStep = C::kStageBytes >> 4;
     const uint64_t dq = smem_desc(smem_u32(smem));
     const uint64_t dk = smem_desc(smem_u32(smem + C::kOffKv)), dv = smem_desc(smem_u32(smem + C::kOffKv), C::kSub);
+    const uint32_t b_full = smem_u32(kv_full), b_empty = smem_u32(kv_empty), b_s = smem_u32(s_full), b_p = smem_u32(p_full),
+                   b_o = smem_u32(o_full), b_q = smem_u32(q_empty);
     uint32_t st = 0, st_par = 0, q_par = 0, p_par0 = 0, p_par1 = 0;
     auto take = [&]() {  // the next stage of the ring, filled
       const uint32_t now = st;
-      wait(&kv_full[now], st_par);
+      wait(b_full + now * 8, st_par);
       if (++st == C::kStages) {
         st = 0;
         st_par ^= 1;
       }
       return now;
     };
-    // O += P V over the first (part 0) or the other tokens of each half of the tile; the halves' P lie 64 columns apart
-    auto pv = [&](int s, uint64_t b, bool acc, int part) {
+    auto pv = [&](int s, uint64_t b, bool acc) {  // the halves' P lie 64 columns apart
 #pragma unroll
       for (int k = 0; k < kTile / 16; ++k)
-        if (((k & 3) * 16 < C::kPart0) == (part == 0))
-          mma_ts(tmem + C::kColO + s * D, tmem + s * kTile + (k >> 2) * 64 + (k & 3) * 8, b + (k * 2048 >> 4), kIdPv,
-                 acc || k > 0);
+        mma_ts(tmem + C::kColO + s * D, tmem + s * kTile + (k >> 2) * 64 + (k & 3) * 8, b + (k * 2048 >> 4), kIdPv, acc || k > 0);
     };
     auto qk = [&](int s, uint64_t a, uint64_t b) {
 #pragma unroll
@@ -290,18 +321,11 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         const uint32_t off = ((k / 4) * (kRows * 128) + (k % 4) * 32) >> 4;
         mma_ss(tmem + s * kTile, a + off, b + off, kIdQk, k > 0);
       }
-      tc_commit(&s_full[s]);
+      tc_commit_at(b_s + s * 8);
     };
-    // waits for stream s's probabilities of a tile and issues their product up to the last part
-    constexpr bool kParts = C::kPart0 < 64;
-    auto pv_first = [&](int s, uint32_t sv, bool acc) {
+    auto wait_p = [&](int s) {
       uint32_t &par = s == 0 ? p_par0 : p_par1;
-      if (kParts) {
-        wait(&p_full[s], par);
-        tc_fence_after();
-        if (elect_one()) pv(s, dv + sv * kStep, acc, 0);
-      }
-      wait(&p_rest[s], par);
+      wait(b_p + s * 8, par);
       par ^= 1;
       tc_fence_after();
     };
@@ -311,29 +335,42 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       wait(q_full, q_par);
       q_par ^= 1;
       if (w.dual) {
-        // V of tile j, then K of tile j + 1; the streams alternate
+        // V of tile j, then K of tile j + 1; the streams alternate.  The next pair of stages is waited for behind stream 0's
+        // products, while they run.
+        uint32_t sv = 0, sk = take();
         for (int j = w.it.tile0 - 1; j < w.it.tile1; ++j) {
           const bool has_v = j >= w.it.tile0, has_k = j + 1 < w.it.tile1;
-          const uint32_t sv = has_v ? take() : 0, sk = has_k ? take() : 0;
+          const bool av0 = has_v && j < w.j1[0], av1 = has_v && j >= w.j0[1];
+          const bool ak0 = has_k && j + 1 < w.j1[0], ak1 = has_k && j + 1 >= w.j0[1];
           tc_fence_after();
-#pragma unroll
-          for (int s = 0; s < 2; ++s) {
-            const bool av = has_v && j >= w.j0[s] && j < w.j1[s], ak = has_k && j + 1 >= w.j0[s] && j + 1 < w.j1[s];
-            if (av) pv_first(s, sv, j > w.j0[s]);
-            if (elect_one()) {
-              if (av) {
-                pv(s, dv + sv * kStep, kParts || j > w.j0[s], kParts ? 1 : 0);
-                if (j + 1 == w.j1[s]) tc_commit(&o_full[s]);
-              }
-              if (s == 1 && has_v) tc_commit(&kv_empty[sv]);
-              if (ak) qk(s, dq + s * (C::kQBytes >> 4), dk + sk * kStep);
-              if (s == 1 && has_k) {
-                tc_commit(&kv_empty[sk]);
-                if (j + 2 >= w.it.tile1) tc_commit(q_empty);
-              }
+          if (av0) wait_p(0);
+          if (elect_one()) {
+            if (av0) {
+              pv(0, dv + sv * kStep, j > w.j0[0]);
+              if (j + 1 == w.j1[0]) tc_commit_at(b_o);
             }
-            __syncwarp();
+            if (ak0) qk(0, dq, dk + sk * kStep);
           }
+          __syncwarp();
+          uint32_t nv = 0, nk = 0;
+          if (has_k) nv = take();
+          if (j + 2 < w.it.tile1) nk = take();
+          if (av1) wait_p(1);
+          if (elect_one()) {
+            if (av1) {
+              pv(1, dv + sv * kStep, j > w.j0[1]);
+              if (j + 1 == w.j1[1]) tc_commit_at(b_o + 8);
+            }
+            if (has_v) tc_commit_at(b_empty + sv * 8);
+            if (ak1) qk(1, dq + (C::kQBytes >> 4), dk + sk * kStep);
+            if (has_k) {
+              tc_commit_at(b_empty + sk * 8);
+              if (j + 2 >= w.it.tile1) tc_commit_at(b_q);
+            }
+          }
+          __syncwarp();
+          sv = nv;
+          sk = nk;
         }
       } else {
         // V of tile i, then K of tile i + 2, both on stream i & 1
@@ -344,17 +381,17 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
 #pragma unroll
           for (int s = 0; s < 2; ++s) {
             if ((i & 1) != s) continue;
-            if (has_v) pv_first(s, sv, i > 1);
+            if (has_v) wait_p(s);
             if (elect_one()) {
               if (has_v) {
-                pv(s, dv + sv * kStep, kParts || i > 1, kParts ? 1 : 0);
-                if (i + 2 >= w.n) tc_commit(&o_full[s]);
-                tc_commit(&kv_empty[sv]);
+                pv(s, dv + sv * kStep, i > 1);
+                if (i + 2 >= w.n) tc_commit_at(b_o + s * 8);
+                tc_commit_at(b_empty + sv * 8);
               }
               if (has_k) {
                 qk(s, dq, dk + sk * kStep);
-                tc_commit(&kv_empty[sk]);
-                if (i + 3 == w.n) tc_commit(q_empty);
+                tc_commit_at(b_empty + sk * 8);
+                if (i + 3 == w.n) tc_commit_at(b_q);
               }
             }
             __syncwarp();
@@ -365,7 +402,67 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     if (elect_one()) tc_commit(fin);  // every arrival that the instructions still owe has happened before the block ends
     __syncwarp();
     wait(fin, 0);
-  } else if (warp >= 4) {
+  } else if (warp < 4) {
+    if constexpr (KV8) {
+      // ------------------------------------------------------------------ int8 tiles to fp16, half a tile per warp
+      // A byte u = x + 128 under 0x64 is the fp16 1024 + u, exactly; 1152 taken off gives x.
+      uint32_t c = 0;
+      const int r_first = (warp - 2) * (kTile / 2);
+      for (int r = 0, item = item_of(0); item < p.items; item = item_of(++r)) {
+        const Work w = make_work(seqs, p, item);
+        if (w.n == 0) continue;
+        const ChunkSeq &e = seqs.s[w.it.seq];
+        const int alive0 = p.window > 0 ? max(0, e.ctx - e.q_len - p.window + 1) : 0, alive1 = e.ctx;
+        auto convert = [&](int j) {
+          const uint32_t rs = c % C::kRaw, st = c % C::kStages, raw_use = c / C::kRaw, use = c / C::kStages;
+          ++c;
+          wait(&raw_full[rs], raw_use & 1);
+          if (use > 0) wait(&kv_empty[st], (use - 1) & 1);
+          const uint8_t *src = smem + C::kOffRaw + rs * C::kRawBytes;
+          uint8_t *dst = smem + C::kOffKv + st * C::kStageBytes;
+          const int tok = j * kTile;
+          const int a = max(0, alive0 - tok), b = min(kTile, alive1 - tok);  // rows that are alive; the others become zero
+          constexpr int kPieces = D / 16;  // 16-byte pieces of a raw row
+  #pragma unroll 4
+          for (int i = lane; i < kTile / 2 * kPieces; i += 32) {
+            const int row = r_first + i / kPieces, pc = i % kPieces;
+            uint4 v = *reinterpret_cast<const uint4 *>(src + row * D + pc * 16);
+            if (row < a || row >= b) v = make_uint4(0, 0, 0, 0);
+            uint32_t o[8];
+            const uint32_t in[4] = {v.x, v.y, v.z, v.w};
+  #pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const uint32_t u = in[k] ^ 0x80808080u;
+              const __half2 bias = __half2half2(__ushort_as_half(0x6480));  // 1152
+              uint32_t lo = __byte_perm(u, 0x64646464u, 0x4140), hi = __byte_perm(u, 0x64646464u, 0x4342);
+              __half2 l2 = __hsub2(*reinterpret_cast<__half2 *>(&lo), bias), h2 = __hsub2(*reinterpret_cast<__half2 *>(&hi), bias);
+              o[2 * k] = *reinterpret_cast<uint32_t *>(&l2);
+              o[2 * k + 1] = *reinterpret_cast<uint32_t *>(&h2);
+            }
+            // two 16-byte chunks of the swizzled row; lanes of the second sub-tile write theirs in the other order, so that
+            // the eight lanes of a row hit eight different chunks
+            uint8_t *base = dst + (pc / 4) * C::kSub + row * 128;
+            const int ch = (pc % 4) * 2, odd = (pc / 4) & 1;
+            const uint4 c0 = make_uint4(o[0], o[1], o[2], o[3]), c1 = make_uint4(o[4], o[5], o[6], o[7]);
+            *reinterpret_cast<uint4 *>(base + (((ch + odd) ^ (row & 7)) << 4)) = odd ? c1 : c0;
+            *reinterpret_cast<uint4 *>(base + (((ch + 1 - odd) ^ (row & 7)) << 4)) = odd ? c0 : c1;
+          }
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(&kv_full[st]);
+            mbar_arrive(&raw_empty[rs]);
+          }
+        };
+        const int ahead = w.step;
+        for (int i = 0; i < min(ahead, w.n); ++i) convert(w.it.tile0 + i);
+        for (int i = 0; i < w.n; ++i) {
+          convert(w.it.tile0 + i);
+          if (i + ahead < w.n) convert(w.it.tile0 + i + ahead);
+        }
+      }
+    }
+  } else {
     // ------------------------------------------------------------------ softmax, two threads per row
     // The threads of a row are in two warps, one for each half of a tile's columns (and of O's): with four softmax warps
     // on each scheduler the latencies of one hide behind the others.  They exchange their halves' maxima.
@@ -391,7 +488,62 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       const int pos = live ? pos0 + tok_in : -1;
       const int j_beg = s == 0 ? w.j0[0] : w.j0[1], j_end = s == 0 ? w.j1[0] : w.j1[1];
       float m = -INFINITY, l = 0.f;
-      if (speaker && w.n > 0) {
+      float sc = p.scale_log2e;  // score -> log2 domain
+      float shift = 0.f;         // int8 with offsets: the part of a row's scores that all tokens share (for the lse)
+      if (KV8 && w.n > 0) {
+        // Q' = q * k_descale, scaled by a power of two to a largest magnitude of 2^13 .. 2^14 and rounded to fp16 (2^-11 of
+        // each, whatever the scales), into this stream's tile (single: stream 0's).  The tile is free: this stream's products
+        // of the item in front are complete, and those of the other on the same tile by the merge.
+        if (w.dual || s == 0) {
+          float top = 0.f, off = 0.f;
+          const T *src = static_cast<const T *>(p.q) +
+                         (((int64_t)e.q_start + tok0 + tok_in) * p.num_q_heads + w.it.kvh * g + head_in) * D + hf * (D / 2);
+          const float *ds = p.k_descale + w.it.kvh * D + hf * (D / 2);
+          const int32_t *of = p.k_offset == nullptr ? nullptr : p.k_offset + w.it.kvh * D + hf * (D / 2);
+          float q[D / 2];
+#pragma unroll
+          for (int c = 0; c < D / 2; c += 8) {
+            uint4 v = live ? __ldg(reinterpret_cast<const uint4 *>(src + c)) : make_uint4(0, 0, 0, 0);
+            const T *qe = reinterpret_cast<const T *>(&v);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              q[c + i] = to_f32(qe[i]) * __ldg(ds + c + i);
+              top = fmaxf(top, fabsf(q[c + i]));
+              if (of != nullptr) off = fmaf(q[c + i], (float)__ldg(of + c + i), off);
+            }
+          }
+          *x_mine = top;
+          named_bar_sync(pair, 64);
+          top = fmaxf(top, *x_other);
+          named_bar_sync(pair, 64);
+          if (of != nullptr) {
+            *x_mine = off;
+            named_bar_sync(pair, 64);
+            off += *x_other;
+            named_bar_sync(pair, 64);
+          }
+          const int ex = min(max((int)(__float_as_uint(top) >> 23) - 127, -113), 128);  // exponent of the largest
+          const float up = top > 0.f ? __uint_as_float((uint32_t)(127 + 13 - ex) << 23) : 1.f;
+          uint8_t *dst = smem + (w.dual ? s * C::kQBytes : 0) + row * 128;
+#pragma unroll
+          for (int c = 0; c < D / 2; c += 8) {
+            const int col = hf * (D / 2) + c;
+            const uint4 v = make_uint4(pack2<M>(q[c] * up, q[c + 1] * up), pack2<M>(q[c + 2] * up, q[c + 3] * up),
+                                       pack2<M>(q[c + 4] * up, q[c + 5] * up), pack2<M>(q[c + 6] * up, q[c + 7] * up));
+            *reinterpret_cast<uint4 *>(dst + (col / 64) * (kRows * 128) + ((((col % 64) / 8) ^ (row & 7)) << 4)) = v;
+          }
+          sc = p.scale_log2e / up;
+          shift = off * p.scale_log2e;
+          if (!w.dual && hf == 0) q_scale[row] = sc;
+          fence_proxy_async();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(q_full);
+        wait(q_full, q_round & 1);  // (single: stream 1 takes its rows' scales from stream 0; and nobody runs ahead)
+        ++q_round;
+        if (!w.dual && s == 1) sc = q_scale[row];
+      }
+      if (!KV8 && speaker && w.n > 0) {
         // One of the two arrivals that free Q's space is stream 1's: at once (dual), or when the merge is through with it
         // (single).  It comes behind the arrival of the item's rows, so never before the one of the item in front.
         wait(q_full, q_round & 1);
@@ -427,10 +579,10 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
 #pragma unroll
           for (int i = 0; i < 4; ++i) mx4[i] = fmaxf(mx4[i], __uint_as_float(x[60 + i]));
           float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
-          // (the next tile's exchange comes behind that tile's s_full, which both warps' p_rest of this one precede)
+          // (the next tile's exchange comes behind that tile's s_full, which both warps' p_full of this one precede)
           *x_mine = mx;
           named_bar_sync(pair, 64);
-          mx = fmaxf(mx, *x_other) * p.scale_log2e;
+          mx = fmaxf(mx, *x_other) * sc;
           const bool first = j == j_beg;
           const bool grow = mx > m + kSlack;  // also for the first value: m is -inf
           if (__any_sync(0xffffffffu, grow)) {
@@ -450,7 +602,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
             }
           }
           const float base = m == -INFINITY ? 0.f : m;
-          const uint64_t scale2 = pack_f32x2(p.scale_log2e, p.scale_log2e), base2 = pack_f32x2(-base, -base);
+          const uint64_t scale2 = pack_f32x2(sc, sc), base2 = pack_f32x2(-base, -base);
           uint64_t sum2[2] = {0, 0};
 #pragma unroll
           for (int c0 = 0; c0 < 64; c0 += 32) {
@@ -467,27 +619,20 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
                 b = fast_exp2(b);
               }
               sum2[(i >> 1) & 1] = add_f32x2(sum2[(i >> 1) & 1], pack_f32x2(a, b));
-              pk[i / 2] = pack2<T>(a, b);
+              pk[i / 2] = pack2<M>(a, b);
             }
             tmem_st16(t_s + c0 / 2, pk);
-            if (c0 + 32 == C::kPart0 && C::kPart0 < 64) {  // the product may start on these tokens
-              tc_wait_st();
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&p_full[s]);
-            }
           }
           tc_wait_st();
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&p_rest[s]);
+          if (lane == 0) mbar_arrive(&p_full[s]);
           float s0, s1;
           unpack_f32x2(add_f32x2(sum2[0], sum2[1]), s0, s1);
           l += s0 + s1;
           if (m == -INFINITY) l = 0.f;  // nothing seen so far: the polynomial's 2^-126 does not count
         } else if (lane == 0) {
-          if (C::kPart0 < 64) mbar_arrive(&p_full[s]);
-          mbar_arrive(&p_rest[s]);
+          mbar_arrive(&p_full[s]);
         }
       }
       // ---- the item's result
@@ -565,7 +710,14 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
             } else {
               uint32_t pk[8];
 #pragma unroll
-              for (int i = 0; i < 8; ++i) pk[i] = pack2<T>(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
+              for (int i = 0; i < 8; ++i) {
+                float a = __uint_as_float(o[2 * i]) * inv, b = __uint_as_float(o[2 * i + 1]) * inv;
+                if (KV8) {
+                  a = dequant_out(p, w.it.kvh * D + col + 2 * i, a, inv);
+                  b = dequant_out(p, w.it.kvh * D + col + 2 * i + 1, b, inv);
+                }
+                pk[i] = pack2<T>(a, b);
+              }
               store_32b(static_cast<T *>(p.out) + orow * D + col, pk);
             }
           }
@@ -576,8 +728,9 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         }
       }
       // the merge buffer lies over Q's second tile: only now may the next item's rows come in
-      if (speaker && w.n > 0 && !w.dual && lane == 0) mbar_arrive(q_empty);
+      if (!KV8 && speaker && w.n > 0 && !w.dual && lane == 0) mbar_arrive(q_empty);
       if (writes && hf == 0) {
+        m_out += shift;
         if (split) *reinterpret_cast<float2 *>(p.part_ml + prow * 2) = make_float2(m_out, l_out);
         else if (p.lse != nullptr) p.lse[orow] = l_out > 0.f ? (m_out + log2f(l_out)) * kLn2 : -INFINITY;
       }
@@ -637,7 +790,14 @@ __global__ void __launch_bounds__(256) chunk_merge_kernel(const __grid_constant_
     const int64_t orow = ((int64_t)e.q_start + tok) * p.num_q_heads + hq;
     uint32_t *dst = reinterpret_cast<uint32_t *>(static_cast<T *>(p.out) + orow * D + lane * kCols);
 #pragma unroll
-    for (int c = 0; c < kCols; c += 2) dst[c / 2] = pack2<T>(acc[c] * inv, acc[c + 1] * inv);
+    for (int c = 0; c < kCols; c += 2) {
+      float a = acc[c] * inv, b = acc[c + 1] * inv;
+      if (p.v_descale != nullptr) {
+        a = dequant_out(p, kvh * D + lane * kCols + c, a, inv);
+        b = dequant_out(p, kvh * D + lane * kCols + c + 1, b, inv);
+      }
+      dst[c / 2] = pack2<T>(a, b);
+    }
     if (lane == 0 && p.lse != nullptr) p.lse[orow] = l > 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
   }
 }
@@ -658,27 +818,29 @@ EncodeTiledFn encode_fn() {
   return fn;
 }
 
-int encode(CUtensorMap *tm, const void *base, int32_t dtype, const cuuint64_t (&dims)[3], const cuuint64_t (&strides)[2],
+int encode(CUtensorMap *tm, const void *base, int32_t dtype, bool swizzle, const cuuint64_t (&dims)[3], const cuuint64_t (&strides)[2],
            const cuuint32_t (&box)[3]) {
   EncodeTiledFn fn = encode_fn();
   if (fn == nullptr) return fail(MSCO_ERR_CUDA, "chunk_attention: cuTensorMapEncodeTiled is not available");
   const cuuint32_t one[3] = {1, 1, 1};
-  const CUresult r = fn(tm, dtype == MSCO_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
-                        const_cast<void *>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const CUtensorMapDataType dt = dtype == MSCO_DTYPE_I8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                 : dtype == MSCO_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const CUresult r = fn(tm, dt, 3, const_cast<void *>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(MSCO_ERR_CUDA, "chunk_attention: cuTensorMapEncodeTiled failed (%d)", (int)r);
   return MSCO_OK;
 }
 
-template <typename T, int D, int N>
+template <typename T, int D, bool KV8, int N>
 int launch_sized(const MscoChunkDesc &d, const ChunkParams &p, const ChunkSeq *src, int64_t q_rows, int sms,
                  cudaStream_t stream) {
-  using C = Cfg<D>;
+  using C = Cfg<D, KV8>;
   static_assert(C::kSmem <= 232448, "shared memory of one SM exceeded");
   const cuuint64_t h = (cuuint64_t)d.num_kv_heads, bs = (cuuint64_t)d.block_size, nb = (cuuint64_t)d.num_blocks;
-  const cuuint32_t rows = (cuuint32_t)std::min(d.block_size, kTile);
+  const cuuint64_t row = (cuuint64_t)D * (KV8 ? 1 : 2);  // bytes of one token of one head
+  const cuuint32_t rows = (cuuint32_t)std::min(d.block_size, kTile), cols = KV8 ? (cuuint32_t)D : 64u;
   CUtensorMap tq, tk, tv;
-  int rc = encode(&tq, p.q, d.q_dtype, {(cuuint64_t)D, (cuuint64_t)d.num_q_heads, (cuuint64_t)q_rows},
+  int rc = encode(&tq, p.q, d.q_dtype, true, {(cuuint64_t)D, (cuuint64_t)d.num_q_heads, (cuuint64_t)q_rows},
                   {(cuuint64_t)D * 2, (cuuint64_t)d.num_q_heads * D * 2},
                   {64u, (cuuint32_t)p.group, (cuuint32_t)(p.item_tokens / 2)});
   if (rc != MSCO_OK) return rc;
@@ -686,8 +848,8 @@ int launch_sized(const MscoChunkDesc &d, const ChunkParams &p, const ChunkSeq *s
     const void *cache = i == 0 ? p.key_cache : p.value_cache;
     CUtensorMap *tm = i == 0 ? &tk : &tv;
     rc = d.cache_layout == 1
-             ? encode(tm, cache, d.kv_dtype, {(cuuint64_t)D, bs, nb * h}, {(cuuint64_t)D * 2, bs * D * 2}, {64u, rows, 1u})
-             : encode(tm, cache, d.kv_dtype, {(cuuint64_t)D, h, nb * bs}, {(cuuint64_t)D * 2, h * D * 2}, {64u, 1u, rows});
+             ? encode(tm, cache, d.kv_dtype, !KV8, {(cuuint64_t)D, bs, nb * h}, {row, bs * row}, {cols, rows, 1u})
+             : encode(tm, cache, d.kv_dtype, !KV8, {(cuuint64_t)D, h, nb * bs}, {row, h * row}, {cols, 1u, rows});
     if (rc != MSCO_OK) return rc;
   }
   ChunkSeqs<N> seqs;
@@ -700,7 +862,7 @@ int launch_sized(const MscoChunkDesc &d, const ChunkParams &p, const ChunkSeq *s
       max_rows = std::max<int64_t>(max_rows, (int64_t)src[i].q_len * p.num_q_heads);
     }
   }
-  auto kfn = chunk_tc_kernel<T, D, N>;
+  auto kfn = chunk_tc_kernel<T, D, KV8, N>;
   // set per call: the attribute belongs to a device
   MSCO_CUDA_CHECK(cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
   kfn<<<std::min(p.items, sms), kThreads, C::kSmem, stream>>>(tq, tk, tv, p, seqs);
@@ -720,11 +882,21 @@ int launch_sized(const MscoChunkDesc &d, const ChunkParams &p, const ChunkSeq *s
   return MSCO_OK;
 }
 
-template <typename T, int D>
+template <typename T, int D, bool KV8>
 int launch_typed(const MscoChunkDesc &d, const ChunkParams &p, const ChunkSeq *src, int64_t q_rows, int sms,
                  cudaStream_t stream) {
-  if (p.nseq <= kChunkSeqsSmall) return launch_sized<T, D, kChunkSeqsSmall>(d, p, src, q_rows, sms, stream);
-  return launch_sized<T, D, kChunkSeqsMax>(d, p, src, q_rows, sms, stream);
+  if (p.nseq <= kChunkSeqsSmall) return launch_sized<T, D, KV8, kChunkSeqsSmall>(d, p, src, q_rows, sms, stream);
+  return launch_sized<T, D, KV8, kChunkSeqsMax>(d, p, src, q_rows, sms, stream);
+}
+
+template <typename T>
+int launch_of(const MscoChunkDesc &d, const ChunkParams &p, const ChunkSeq *src, int64_t q_rows, int sms, cudaStream_t stream) {
+  const bool i8 = d.kv_dtype == MSCO_DTYPE_I8;
+  if (d.head_dim == 64)
+    return i8 ? launch_typed<T, 64, true>(d, p, src, q_rows, sms, stream)
+              : launch_typed<T, 64, false>(d, p, src, q_rows, sms, stream);
+  return i8 ? launch_typed<T, 128, true>(d, p, src, q_rows, sms, stream)
+            : launch_typed<T, 128, false>(d, p, src, q_rows, sms, stream);
 }
 
 }  // namespace
@@ -734,18 +906,14 @@ bool chunk_tc_supported(const MscoChunkDesc &d) {
   const int bs = d.block_size;
   const bool bs_ok = bs % kTile == 0 || bs == 8 || bs == 16 || bs == 32 || bs == 64;
   const int group = d.num_q_heads / d.num_kv_heads;
-  return (d.head_dim == 64 || d.head_dim == 128) && bs_ok && group <= kRows && d.kv_dtype == d.q_dtype && d.qk_scale > 0 &&
+  return (d.head_dim == 64 || d.head_dim == 128) && bs_ok && group <= kRows && d.qk_scale > 0 &&
          d.num_blocks * (int64_t)bs < (1ll << 31) && d.num_blocks * (int64_t)d.num_kv_heads < (1ll << 31);
 }
 
 int launch_chunk_tc(const MscoChunkDesc &d, const ChunkParams &p, const ChunkSeq *seqs, int64_t q_rows, int sms,
                     cudaStream_t stream) {
-  const bool f16 = d.q_dtype == MSCO_DTYPE_F16;
-  if (d.head_dim == 64)
-    return f16 ? launch_typed<__half, 64>(d, p, seqs, q_rows, sms, stream)
-               : launch_typed<__nv_bfloat16, 64>(d, p, seqs, q_rows, sms, stream);
-  return f16 ? launch_typed<__half, 128>(d, p, seqs, q_rows, sms, stream)
-             : launch_typed<__nv_bfloat16, 128>(d, p, seqs, q_rows, sms, stream);
+  return d.q_dtype == MSCO_DTYPE_F16 ? launch_of<__half>(d, p, seqs, q_rows, sms, stream)
+                                     : launch_of<__nv_bfloat16>(d, p, seqs, q_rows, sms, stream);
 }
 
 int chunk_tc_status() {

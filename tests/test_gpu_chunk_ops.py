@@ -5,7 +5,10 @@ Tolerances follow from the arithmetic.  With h half a step of the output type (f
                    and their exponential is good to 2^-12 of itself; a score is a float32 sum of head_dim products
                    (head_dim 2^-24 of the sum of their magnitudes, which moves a probability by as much; twice, for
                    numerator and denominator); with an int8 cache the query times the scales is rounded to fp16
-                   (2^-11 of the same sum).  All of it relative to A = sum p |v| / sum p.
+                   (2^-11 of the same sum).  All of it relative to A = sum p |v| / sum p.  With an int8 cache the product
+                   runs over the raw values r and (sum p r / sum p + offset) * descale follows: with p' = p (1 + d),
+                   |d| <= e, it is off by descale |sum p d r| / sum p <= e * sum p |r| descale / sum p, so A is taken over
+                   |r| descale there (the offset carries no error of p).
   rope_and_cache   one rounding (h |y|) of a float32 value that a handful of float32 operations give (8 * 2^-24 of the
                    magnitudes |a c| + |b s|).
 """
@@ -92,14 +95,14 @@ class Chunk:
                                    torch.tensor(self.ctx, dtype=torch.int32), qk_scale=self.scale,
                                    window_size=self.window, input_layout=self.layout, **self.scales, **kw)
 
-    def rows_of(self, cache, name, b, lo, c):
-        """Rows [lo, c) of sequence b in 64 bits, [rows, kv_heads, dim]."""
+    def rows_of(self, cache, name, b, lo, c, raw=False):
+        """Rows [lo, c) of sequence b in 64 bits, [rows, kv_heads, dim]; `raw`: int8 values without their offset."""
         j = torch.arange(lo, c, device="cuda")
         blk = self.full_tables[b].cuda()[j // self.block]
         x = (cache[blk, :, j % self.block] if self.layout else cache[blk, j % self.block]).double()
         if self.int8:
             shape = (self.kv_heads, self.dim)
-            if name + "_offset" in self.scales:
+            if name + "_offset" in self.scales and not raw:
                 x = x + self.scales[name + "_offset"].double().view(shape)
             x = x * self.scales[name + "_descale"].double().view(shape)
         return x
@@ -117,6 +120,7 @@ class Chunk:
             lo = min(lo, c)
             if ql and c:
                 k, v = self.rows_of(self.kc, "k", b, lo, c), self.rows_of(self.vc, "v", b, lo, c)
+                v_mag = self.rows_of(self.vc, "v", b, lo, c, raw=True).abs()
                 j = torch.arange(lo, c, device="cuda")
                 for t0 in range(0, ql, 1024):
                     t1 = min(ql, t0 + 1024)
@@ -133,7 +137,7 @@ class Chunk:
                         p = torch.exp(s - torch.where(some[:, None], top, 0.0))
                         l = p.sum(1, keepdim=True)
                         den = torch.where(some[:, None], l, 1.0)
-                        o, a = p @ vv / den, p @ vv.abs() / den
+                        o, a = p @ vv / den, p @ v_mag[:, hd // grp] / den
                         mag = (q.abs() @ kk.abs().T * abs(self.scale)).masked_fill(~seen, 0).amax(1, keepdim=True)
                         ds = mag * (self.dim * 2.0 ** -24 + (2.0 ** -11 if self.int8 else 0.0))
                         out[at + t0:at + t1, hd] = o
