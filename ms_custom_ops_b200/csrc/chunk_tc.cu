@@ -11,8 +11,8 @@
 // more than kSlack (a factor 256): until then P is up to 256 instead of 1, which costs no precision in a floating
 // format, and O stays where it is; it is rescaled in TMEM by the softmax warps in the rare tiles where it must.
 //
-// Warps: 0 loads (TMA, 128-byte swizzle), 1 matrix instructions, 2 / 3 int8 to fp16 (16-bit caches: idle; registers are
-// handed out by groups of four warps), 4-11 / 12-19 softmax of stream 0 / 1.
+// Warps: 0 loads (TMA, 128-byte swizzle), 1 matrix instructions (2, 3 idle: registers are handed out by groups of four
+// warps); int8 caches: four that convert; then eight of softmax for stream 0, eight for stream 1.
 // The matrix instructions are issued O_0 += P_0 V, S_0 = Q_0 K', O_1 += P_1 V, S_1 = Q_1 K' (K' the next tile); they execute in
 // that order, so a completed S' means that the product that read P, which lies over it, is complete too.
 #include <cuda.h>
@@ -30,7 +30,6 @@ namespace {
 
 constexpr int kRows = 128;        // rows of one stream
 constexpr int kTile = kChunkKvTile;
-constexpr int kThreads = 640;
 constexpr int kSoftWarps = 8;     // per stream
 constexpr float kSlack = 8.f;     // log2 of how far a probability may exceed 1
 constexpr float kLn2 = 0.6931471805599453f;
@@ -41,6 +40,9 @@ __device__ int g_chunk_error;  // MSCO_ERR_TIMEOUT once a bounded wait has run o
 template <int D, bool KV8>
 struct Cfg {
   static_assert(D == 64 || D == 128, "head_dim 64 or 128");
+  // four warps of loads and matrix instructions, four that convert int8 tiles, sixteen of softmax
+  static constexpr int kFirstSoft = KV8 ? 8 : 4;
+  static constexpr int kThreads = (kFirstSoft + 16) * 32;
   static constexpr int kBoxes = D / 64;                 // 128-byte wide sub-tiles of a row
   static constexpr int kSub = kTile * 128;              // bytes of one sub-tile
   static constexpr int kStageBytes = kTile * D * 2;
@@ -148,7 +150,7 @@ __device__ __forceinline__ int item_of(int r) {
 }
 
 template <typename T, int D, bool KV8, int N>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(Cfg<D, KV8>::kThreads, 1)
 chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                 const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ ChunkParams p,
                 const __grid_constant__ ChunkSeqs<N> seqs) {
@@ -169,13 +171,13 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (threadIdx.x == 0) {
     for (int i = 0; i < C::kStages; ++i) {
-      mbar_init(&kv_full[i], KV8 ? 2 : 1);  // the copy, or the two converting warps
+      mbar_init(&kv_full[i], KV8 ? 4 : 1);  // the copy, or the four converting warps
       mbar_init(&kv_empty[i], 1);
     }
     mbar_init(q_full, KV8 ? 2 * kSoftWarps : 1);
     for (int i = 0; i < C::kRaw; ++i) {
       mbar_init(&raw_full[i], 1);
-      mbar_init(&raw_empty[i], 2);
+      mbar_init(&raw_empty[i], 4);
     }
     mbar_init(q_empty, 2);
     for (int s = 0; s < 2; ++s) {
@@ -196,8 +198,11 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   const Waiter wait{abort_flag};
   const int half = p.item_tokens >> 1;
 
-  // Registers: 640 x 96 at launch = 512 x 104 (softmax) + 128 x 64 (the first four warps)
-  if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+  // Registers: 640 x 96 at launch = 512 x 104 (softmax) + 128 x 64, with the converting warps 768 x 80 = 512 x 96 + 256 x 48
+  if (warp < C::kFirstSoft) {
+    if (KV8) asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+  }
   if (warp == 0) {
     // ------------------------------------------------------------------ loads
     if (lane == 0) {
@@ -402,12 +407,13 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     if (elect_one()) tc_commit(fin);  // every arrival that the instructions still owe has happened before the block ends
     __syncwarp();
     wait(fin, 0);
-  } else if (warp < 4) {
+  } else if (warp < C::kFirstSoft) {
     if constexpr (KV8) {
-      // ------------------------------------------------------------------ int8 tiles to fp16, half a tile per warp
+      if (warp >= 4) {
+      // ------------------------------------------------------------------ int8 tiles to fp16, a quarter of a tile per warp
       // A byte u = x + 128 under 0x64 is the fp16 1024 + u, exactly; 1152 taken off gives x.
       uint32_t c = 0;
-      const int r_first = (warp - 2) * (kTile / 2);
+      const int r_first = (warp - 4) * (kTile / 4);
       for (int r = 0, item = item_of(0); item < p.items; item = item_of(++r)) {
         const Work w = make_work(seqs, p, item);
         if (w.n == 0) continue;
@@ -423,29 +429,38 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           const int tok = j * kTile;
           const int a = max(0, alive0 - tok), b = min(kTile, alive1 - tok);  // rows that are alive; the others become zero
           constexpr int kPieces = D / 16;  // 16-byte pieces of a raw row
-  #pragma unroll 4
-          for (int i = lane; i < kTile / 2 * kPieces; i += 32) {
-            const int row = r_first + i / kPieces, pc = i % kPieces;
-            uint4 v = *reinterpret_cast<const uint4 *>(src + row * D + pc * 16);
-            if (row < a || row >= b) v = make_uint4(0, 0, 0, 0);
-            uint32_t o[8];
-            const uint32_t in[4] = {v.x, v.y, v.z, v.w};
-  #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const uint32_t u = in[k] ^ 0x80808080u;
-              const __half2 bias = __half2half2(__ushort_as_half(0x6480));  // 1152
-              uint32_t lo = __byte_perm(u, 0x64646464u, 0x4140), hi = __byte_perm(u, 0x64646464u, 0x4342);
-              __half2 l2 = __hsub2(*reinterpret_cast<__half2 *>(&lo), bias), h2 = __hsub2(*reinterpret_cast<__half2 *>(&hi), bias);
-              o[2 * k] = *reinterpret_cast<uint32_t *>(&l2);
-              o[2 * k + 1] = *reinterpret_cast<uint32_t *>(&h2);
+            constexpr int kBatch = D / 32;  // pieces of a lane that are read before the first is converted
+#pragma unroll 1
+          for (int i0 = lane; i0 < kTile / 4 * kPieces; i0 += 32 * kBatch) {
+            uint4 v[kBatch];
+#pragma unroll
+            for (int n = 0; n < kBatch; ++n) {
+              const int i = i0 + n * 32, row = r_first + i / kPieces;
+              v[n] = *reinterpret_cast<const uint4 *>(src + row * D + i % kPieces * 16);
+              if (row < a || row >= b) v[n] = make_uint4(0, 0, 0, 0);
             }
-            // two 16-byte chunks of the swizzled row; lanes of the second sub-tile write theirs in the other order, so that
-            // the eight lanes of a row hit eight different chunks
-            uint8_t *base = dst + (pc / 4) * C::kSub + row * 128;
-            const int ch = (pc % 4) * 2, odd = (pc / 4) & 1;
-            const uint4 c0 = make_uint4(o[0], o[1], o[2], o[3]), c1 = make_uint4(o[4], o[5], o[6], o[7]);
-            *reinterpret_cast<uint4 *>(base + (((ch + odd) ^ (row & 7)) << 4)) = odd ? c1 : c0;
-            *reinterpret_cast<uint4 *>(base + (((ch + 1 - odd) ^ (row & 7)) << 4)) = odd ? c0 : c1;
+#pragma unroll
+            for (int n = 0; n < kBatch; ++n) {
+              const int i = i0 + n * 32, row = r_first + i / kPieces, pc = i % kPieces;
+              uint32_t o[8];
+              const uint32_t in[4] = {v[n].x, v[n].y, v[n].z, v[n].w};
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const uint32_t u = in[k] ^ 0x80808080u;
+                const __half2 bias = __half2half2(__ushort_as_half(0x6480));  // 1152
+                uint32_t lo = __byte_perm(u, 0x64646464u, 0x4140), hi = __byte_perm(u, 0x64646464u, 0x4342);
+                __half2 l2 = __hsub2(*reinterpret_cast<__half2 *>(&lo), bias), h2 = __hsub2(*reinterpret_cast<__half2 *>(&hi), bias);
+                o[2 * k] = *reinterpret_cast<uint32_t *>(&l2);
+                o[2 * k + 1] = *reinterpret_cast<uint32_t *>(&h2);
+              }
+              // two 16-byte chunks of the swizzled row; lanes of the second sub-tile write theirs in the other order, so
+              // that the eight lanes of a row hit eight different chunks
+              uint8_t *base = dst + (pc / 4) * C::kSub + row * 128;
+              const int ch = (pc % 4) * 2, odd = (pc / 4) & 1;
+              const uint4 c0 = make_uint4(o[0], o[1], o[2], o[3]), c1 = make_uint4(o[4], o[5], o[6], o[7]);
+              *reinterpret_cast<uint4 *>(base + (((ch + odd) ^ (row & 7)) << 4)) = odd ? c1 : c0;
+              *reinterpret_cast<uint4 *>(base + (((ch + 1 - odd) ^ (row & 7)) << 4)) = odd ? c0 : c1;
+            }
           }
           fence_proxy_async();
           __syncwarp();
@@ -461,13 +476,15 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           if (i + ahead < w.n) convert(w.it.tile0 + i + ahead);
         }
       }
+      }
     }
   } else {
     // ------------------------------------------------------------------ softmax, two threads per row
     // The threads of a row are in two warps, one for each half of a tile's columns (and of O's): with four softmax warps
     // on each scheduler the latencies of one hide behind the others.  They exchange their halves' maxima.
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
-    const int s = (warp - 4) >> 3, hf = ((warp >> 2) & 1) ^ 1;
+    if (KV8) asm volatile("setmaxnreg.inc.sync.aligned.u32 96;");
+    else asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+    const int s = (warp - C::kFirstSoft) >> 3, hf = ((warp >> 2) & 1) ^ 1;
     const int row = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)(warp & 3) * 32 << 16;
     const uint32_t t_s = tmem + lanes + s * kTile + hf * 64, t_o = tmem + lanes + C::kColO + s * D + hf * (D / 2);
@@ -865,7 +882,7 @@ int launch_sized(const MscoChunkDesc &d, const ChunkParams &p, const ChunkSeq *s
   auto kfn = chunk_tc_kernel<T, D, KV8, N>;
   // set per call: the attribute belongs to a device
   MSCO_CUDA_CHECK(cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
-  kfn<<<std::min(p.items, sms), kThreads, C::kSmem, stream>>>(tq, tk, tv, p, seqs);
+  kfn<<<std::min(p.items, sms), C::kThreads, C::kSmem, stream>>>(tq, tk, tv, p, seqs);
   MSCO_CUDA_CHECK(cudaGetLastError());
   if (split) {
     cudaLaunchConfig_t cfg = {};
