@@ -97,7 +97,7 @@ __device__ __forceinline__ ChunkItem chunk_item(const ChunkSeqs<N> &seqs, const 
 
 // launchers (defined next to the kernels)
 bool chunk_tc_supported(const MscoChunkDesc &d);
-int launch_chunk_tc(const MscoChunkDesc &d, const ChunkParams &p, const ChunkSeq *seqs, int64_t q_rows, int sms,
+int launch_chunk_tc(const MscoChunkDesc &d, const ChunkParams &p, const ChunkSeq *seqs, int64_t q_rows,
                     cudaStream_t stream);
 int chunk_tc_status();  // MSCO_OK, or MSCO_ERR_TIMEOUT once a bounded wait ran out on the current device (synchronises)
 int launch_chunk_generic(const MscoChunkDesc &d, const ChunkParams &p, const ChunkSeq *seqs, cudaStream_t stream);

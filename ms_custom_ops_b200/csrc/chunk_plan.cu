@@ -2,6 +2,7 @@
 #include <algorithm>
 #include <cmath>
 #include <exception>
+#include <utility>
 #include <vector>
 
 #include "chunk_params.h"
@@ -31,7 +32,7 @@ int check_desc(const MscoChunkDesc &d) {
   return MSCO_OK;
 }
 
-// The sequences with new tokens, those that see most first: their items are the longest and start first.
+// The sequences with new tokens.
 int collect(const MscoChunkDesc &d, const int32_t *q_lens, const int32_t *ctx, int32_t batch,
             std::vector<ChunkSeq> *out) {
   if (batch < 0 || (batch > 0 && (q_lens == nullptr || ctx == nullptr)))
@@ -50,7 +51,6 @@ int collect(const MscoChunkDesc &d, const int32_t *q_lens, const int32_t *ctx, i
     if (q_lens[b] > 0) out->push_back({0, (int32_t)rows, q_lens[b], ctx[b], b, 1, 0x7fffffff, 0});
     rows += q_lens[b];
   }
-  std::stable_sort(out->begin(), out->end(), [](const ChunkSeq &a, const ChunkSeq &b) { return a.ctx > b.ctx; });
   return MSCO_OK;
 }
 
@@ -59,7 +59,7 @@ int item_tokens_of(const MscoChunkDesc &d) { return 2 * (kChunkKvTile / (d.num_q
 
 // KV splits of the tensor-core kernel.  A function of the sequence's own lengths and of the head counts, so that the
 // result of a sequence does not depend on the others of the call.
-void split_rule(const MscoChunkDesc &d, ChunkSeq *e) {
+void split_rule(const MscoChunkDesc &d, ChunkSeq *e, int64_t *cost) {
   const int group = d.num_q_heads / d.num_kv_heads, it = item_tokens_of(d);
   const int64_t alone = (int64_t)((e->q_len + it - 1) / it) * d.num_kv_heads;  // items without splits
   // KV tiles of the longest item
@@ -67,13 +67,25 @@ void split_rule(const MscoChunkDesc &d, ChunkSeq *e) {
   const int hi = e->ctx, lo = d.window > 0 ? std::max(0, e->ctx - e->q_len + last0 - d.window + 1) : 0;
   const int tiles = hi > lo ? (hi + kChunkKvTile - 1) / kChunkKvTile - lo / kChunkKvTile : 0;
   const int rows = std::min(e->q_len, it) * group;
-  const int min_tiles = rows <= 32 ? 4 : (rows <= 128 ? 8 : 24);
-  const int64_t want = std::max<int64_t>(1, 296 / alone);
-  const int nsplit = (int)std::max<int64_t>(1, std::min<int64_t>(want, tiles / min_tiles));
+  const bool dual = rows > kChunkKvTile;
+  // The count that ends first when the sequence has the GPU (148 SMs) to itself: rounds of items times an item's tiles and
+  // what an item costs besides, in tiles (its rows' partial results are written and read again; few rows: little).
+  const int fixed = rows <= 32 ? 2 : (dual ? 6 : 4), most = std::max(1, tiles / (rows <= 32 ? 4 : 8));
+  int nsplit = 1;
+  int64_t best = INT64_MAX;
+  for (int ns = 1; ns <= most && alone * ns <= 148 * 4; ++ns) {
+    const int64_t cost = (alone * ns + 147) / 148 * ((tiles + ns - 1) / ns + (ns > 1 ? fixed : fixed / 2));
+    if (cost < best) {
+      best = cost;
+      nsplit = ns;
+    }
+  }
   e->chunk = nsplit > 1 ? (tiles + nsplit - 1) / nsplit : 0x3fffffff;
   e->nsplit = nsplit > 1 ? (tiles + e->chunk - 1) / e->chunk : 1;
   // windows: an earlier item may touch one tile more than the last one
   if (e->nsplit > 1 && d.window > 0) e->nsplit += 1;
+  // what the longest item takes, for the order: streams share the tiles of a single item
+  *cost = (int64_t)std::min(tiles, e->chunk) * (dual ? 2 : 1);
 }
 
 struct Plan {
@@ -87,10 +99,20 @@ int make_plan(const MscoChunkDesc &d, const int32_t *q_lens, const int32_t *ctx,
   for (const ChunkSeq &e : pl->seqs) pl->q_rows += e.q_len;
   if (!use_tc(d)) return MSCO_OK;
   const int it = item_tokens_of(d), group = d.num_q_heads / d.num_kv_heads;
+  std::vector<std::pair<int64_t, ChunkSeq>> order;
+  order.reserve(pl->seqs.size());
+  for (ChunkSeq &e : pl->seqs) {
+    int64_t cost = 0;
+    split_rule(d, &e, &cost);
+    order.push_back({cost, e});
+  }
+  // the longest items first: the blocks take them in this order
+  std::stable_sort(order.begin(), order.end(),
+                   [](const auto &a, const auto &b) { return a.first > b.first; });
+  for (size_t i = 0; i < order.size(); ++i) pl->seqs[i] = order[i].second;
   for (size_t i = 0; i < pl->seqs.size(); ++i) {
     if (i % kChunkSeqsMax == 0) pl->items.push_back(0);
     ChunkSeq &e = pl->seqs[i];
-    split_rule(d, &e);
     const int64_t tiles = ((int64_t)e.q_len + it - 1) / it * e.nsplit * d.num_kv_heads;
     e.item_base = (int32_t)pl->items.back();
     pl->items.back() += tiles;
@@ -119,15 +141,6 @@ int workspace_bytes_of(const MscoChunkDesc *desc, const int32_t *q_lens, const i
   if (int rc = make_plan(*desc, q_lens, ctx, batch, &pl)) return rc;
   *bytes = bytes_of(*desc, pl);
   return MSCO_OK;
-}
-
-int sm_count() {
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) == cudaSuccess && cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess &&
-      n > 0)
-    return n;
-  (void)cudaGetLastError();
-  return 148;
 }
 
 int launch(const MscoChunkDesc *desc, const int32_t *q_lens, const int32_t *ctx, int32_t batch, const void *query,
@@ -168,12 +181,11 @@ int launch(const MscoChunkDesc *desc, const int32_t *q_lens, const int32_t *ctx,
           reinterpret_cast<uintptr_t>(value_cache)) & 15) != 0 || (reinterpret_cast<uintptr_t>(out) & 31) != 0)
       tc = false;  // rows that the copies cannot start on: the general kernel takes them
   }
-  const int sms = tc ? sm_count() : 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   for (size_t at = 0; at < pl.seqs.size(); at += kChunkSeqsMax) {
     p.nseq = (int)std::min<size_t>(kChunkSeqsMax, pl.seqs.size() - at);
     if (tc) p.items = (int)pl.items[at / kChunkSeqsMax];
-    if (int rc = tc ? launch_chunk_tc(d, p, pl.seqs.data() + at, pl.q_rows, sms, st)
+    if (int rc = tc ? launch_chunk_tc(d, p, pl.seqs.data() + at, pl.q_rows, st)
                     : launch_chunk_generic(d, p, pl.seqs.data() + at, st))
       return rc;
   }

@@ -11,8 +11,8 @@
 // more than kSlack (a factor 256): until then P is up to 256 instead of 1, which costs no precision in a floating
 // format, and O stays where it is; it is rescaled in TMEM by the softmax warps in the rare tiles where it must.
 //
-// Warps: 0 loads (TMA, 128-byte swizzle), 1 matrix instructions (2, 3 idle: registers are handed out by groups of four
-// warps); int8 caches: four that convert; then eight of softmax for stream 0, eight for stream 1.
+// Warps: 0 loads (TMA, 128-byte swizzle), 1 matrix instructions, 2 nothing (registers are handed out by groups of four
+// warps), 3 the next items; int8 caches: four that convert; then eight of softmax for stream 0, eight for stream 1.
 // The matrix instructions are issued O_0 += P_0 V, S_0 = Q_0 K', O_1 += P_1 V, S_1 = Q_1 K' (K' the next tile); they execute in
 // that order, so a completed S' means that the product that read P, which lies over it, is complete too.
 #include <cuda.h>
@@ -54,8 +54,9 @@ struct Cfg {
   static constexpr int kOffKv = 2 * kQBytes;
   static constexpr int kOffRaw = kOffKv + kStages * kStageBytes;
   static constexpr int kOffBar = kOffRaw + kRaw * kRawBytes;
-  static constexpr int kNumBars = 2 * kStages + 2 * kRaw + 10;
-  static constexpr int kOffXch = kOffBar + kNumBars * 8 + 16;  // [stream][half][row]: what the two threads of a row exchange
+  static constexpr int kNumBars = 2 * kStages + 2 * kRaw + 26;
+  static constexpr int kOffResp = (kOffBar + kNumBars * 8 + 16 + 15) / 16 * 16;  // answers of the launch control
+  static constexpr int kOffXch = kOffResp + 32;  // [stream][half][row]: what the two threads of a row exchange
   static constexpr int kSmem = kOffXch + 2 * 2 * kRows * 4 + (KV8 ? kRows * 4 : 0);
   // Of eight pairs of probabilities, those whose exponentials the FMA pipe computes.  At head_dim 128 the special-function
   // unit alone (1024 clocks a tile and stream) is as long as the two products: 2 of 8 took the prompt of 8192 tokens from
@@ -65,7 +66,7 @@ struct Cfg {
 };
 
 // A bounded wait on an mbarrier.  Should one run out (a lost arrival), the block's flag is set, every wait of the block
-// returns at once from then on, and all roles run through the rest of their loops without waiting: whatever they do
+// returns at once from then on, and all roles leave after their item, without waiting: whatever they do
 // stays inside their buffers, the result is worthless and the device's error word says so.
 __device__ __forceinline__ bool mbar_try_wait_at(uint32_t bar, uint32_t parity) {
   uint32_t ok;
@@ -75,6 +76,9 @@ __device__ __forceinline__ bool mbar_try_wait_at(uint32_t bar, uint32_t parity) 
       : "r"(bar), "r"(parity)
       : "memory");
   return ok != 0;
+}
+__device__ __forceinline__ void mbar_arrive_at(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 struct Waiter {
   volatile int *abort;
@@ -143,11 +147,34 @@ __device__ __forceinline__ Work make_work(const ChunkSeqs<N> &seqs, const ChunkP
   return w;
 }
 
-// item of round `r` of this CTA: rounds go forth and back over the CTAs (the list is longest first)
-__device__ __forceinline__ int item_of(int r) {
-  const int g = (int)gridDim.x, c = (int)blockIdx.x;
-  return r * g + ((r & 1) ? g - 1 - c : c);
-}
+// The grid has a block per item, longest first; a running block takes further items by cancelling blocks that have not
+// started (cluster launch control), so that whoever is free takes the next longest.  One warp asks, two answers ahead at
+// most; every other working warp reads each answer and says so.
+struct Items {
+  uint32_t resp, full, empty;  // shared addresses: 16-byte answers [2], mbarriers [2] each
+  int item;
+  uint32_t n;                  // answers read so far
+  template <typename W>
+  __device__ __forceinline__ bool next(const W &wait, int lane) {
+    const uint32_t slot = n & 1;
+    wait(full + slot * 8, (n >> 1) & 1);
+    if (*wait.abort) return false;
+    ++n;
+    uint32_t ok, x;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b128 h;\n\tld.shared.b128 h, [%2];\n\t"
+        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\tselp.u32 %0, 1, 0, p;\n\tmov.u32 %1, 0;\n\t"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, _, _, _}, h;\n\t}"
+        : "=r"(ok), "=r"(x)
+        : "r"(resp + slot * 16)
+        : "memory");
+    fence_proxy_async();  // the answer's place is written next by the asynchronous proxy
+    __syncwarp();
+    if (lane == 0) mbar_arrive_at(empty + slot * 8);
+    item = (int)x;
+    return ok != 0;
+  }
+};
 
 template <typename T, int D, bool KV8, int N>
 __global__ void __launch_bounds__(Cfg<D, KV8>::kThreads, 1)
@@ -162,7 +189,8 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   uint64_t *bars = reinterpret_cast<uint64_t *>(smem + C::kOffBar);
   uint64_t *kv_full = bars, *kv_empty = bars + C::kStages;
   uint64_t *q_full = bars + 2 * C::kStages, *q_empty = q_full + 1, *s_full = q_full + 2, *p_full = q_full + 4,
-           *o_full = q_full + 6, *tail = q_full + 8, *fin = q_full + 9, *raw_full = q_full + 10, *raw_empty = raw_full + C::kRaw;
+           *o_full = q_full + 6, *tail = q_full + 8, *fin = q_full + 9, *clc_full = q_full + 10, *clc_empty = q_full + 12,
+           *m_free = q_full + 14, *pair_bars = q_full + 16, *merge_bar = q_full + 24, *q_full2 = q_full + 25, *raw_full = q_full + 26, *raw_empty = raw_full + C::kRaw;
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + C::kNumBars);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
   float *xch = reinterpret_cast<float *>(smem + C::kOffXch);
@@ -174,18 +202,26 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       mbar_init(&kv_full[i], KV8 ? 4 : 1);  // the copy, or the four converting warps
       mbar_init(&kv_empty[i], 1);
     }
-    mbar_init(q_full, KV8 ? 2 * kSoftWarps : 1);
+    mbar_init(q_full, KV8 ? 2 * kSoftWarps : 1);   // even items
+    mbar_init(q_full2, KV8 ? 2 * kSoftWarps : 1);  // odd items
     for (int i = 0; i < C::kRaw; ++i) {
       mbar_init(&raw_full[i], 1);
       mbar_init(&raw_empty[i], 4);
     }
-    mbar_init(q_empty, 2);
+    mbar_init(q_empty, 1);
     for (int s = 0; s < 2; ++s) {
       mbar_init(&s_full[s], 1);
       mbar_init(&p_full[s], kSoftWarps);
       mbar_init(&o_full[s], 1);
     }
     mbar_init(tail, 1);
+    for (int i = 0; i < 8; ++i) mbar_init(&pair_bars[i], 2);
+    mbar_init(merge_bar, 2 * kSoftWarps);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&clc_full[i], 1);
+      mbar_init(&clc_empty[i], 2 + 16 + (KV8 ? 4 : 0));  // loads, matrix instructions, softmax, conversion
+      mbar_init(&m_free[i], 1);
+    }
     mbar_init(fin, 1);
     *abort_flag = 0;
     fence_barrier_init();
@@ -197,6 +233,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   const uint32_t tmem = *tmem_slot;
   const Waiter wait{abort_flag};
   const int half = p.item_tokens >> 1;
+  const Items items = {smem_u32(smem + C::kOffResp), smem_u32(clc_full), smem_u32(clc_empty), (int)blockIdx.x, 0};
 
   // Registers: 640 x 96 at launch = 512 x 104 (softmax) + 128 x 64, with the converting warps 768 x 80 = 512 x 96 + 256 x 48
   if (warp < C::kFirstSoft) {
@@ -213,23 +250,32 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     const int bs = p.block_size;
     const int box_rows = min(bs, kTile), boxes = kTile / box_rows;
     uint32_t c = 0, q_round = 0, tails = 0;  // ring position, items so far, waits on `tail` so far
-    for (int r = 0, item = item_of(0); item < p.items; item = item_of(++r)) {
-      const Work w = make_work(seqs, p, item);
+    for (Items it = items; it.item >= 0; it.item = it.next(wait, lane) ? it.item : -1) {
+      const Work w = make_work(seqs, p, it.item);
       if (w.n == 0) continue;
       const ChunkSeq &e = seqs.s[w.it.seq];
       // cached tokens that some new token of the sequence sees: the rest of the table may hold anything
       const int alive0 = p.window > 0 ? max(0, e.ctx - e.q_len - p.window + 1) : 0, alive1 = e.ctx;
       const int32_t *table = p.block_tables + (int64_t)e.row * p.max_blocks_per_seq;
-      if (!KV8 && q_round > 0) wait(q_empty, (q_round - 1) & 1);
-      ++q_round;
-      if (!KV8 && lane == 0) {  // (int8: the softmax warps fold the scales into the query rows)
-        const int tiles = w.dual ? 2 : 1;
-        mbar_arrive_expect_tx(q_full, (uint32_t)(tiles * C::kBoxes * half * p.group * 128));
-        for (int s = 0; s < tiles; ++s)
-          for (int x = 0; x < C::kBoxes; ++x)
-            tma_load_3d(smem + s * C::kQBytes + x * (kRows * 128), &tm_q, x * 64, w.it.kvh * p.group,
-                        e.q_start + (s == 0 ? w.it.tok0 : w.t1), q_full);
-      }
+      // The item's query rows.  Their space is free when the last products on them are complete; its second tile also holds
+      // the merge of the two streams of a single item, so a dual item waits for the one in front to be through with that.
+      const uint32_t k_item = q_round++;
+      auto load_q = [&]() {
+        if (KV8) return;  // the softmax warps fold the scales into them
+        if (k_item >= 1) wait(q_empty, (k_item - 1) & 1);
+        if (k_item >= 2) wait(&m_free[k_item & 1], ((k_item - 2) >> 1) & 1);
+        if (w.dual && k_item >= 1) wait(&m_free[(k_item - 1) & 1], ((k_item - 1) >> 1) & 1);
+        uint64_t *bar = k_item & 1 ? q_full2 : q_full;
+        if (lane == 0) {
+          const int tiles = w.dual ? 2 : 1;
+          mbar_arrive_expect_tx(bar, (uint32_t)(tiles * C::kBoxes * half * p.group * 128));
+          for (int s = 0; s < tiles; ++s)
+            for (int x = 0; x < C::kBoxes; ++x)
+              tma_load_3d(smem + s * C::kQBytes + x * (kRows * 128), &tm_q, x * 64, w.it.kvh * p.group,
+                          e.q_start + (s == 0 ? w.it.tok0 : w.t1), bar);
+        }
+        __syncwarp();
+      };
       int win = -1;        // first block-table column of the 32 ids that the lanes hold
       int32_t id = 0;
       // one tile of K or V into the next stage of the ring
@@ -285,12 +331,19 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           if (lane == 0) mbar_arrive(&kv_full[st]);
         }
       };
-      // the order in which the tiles are used: V of a tile right in front of the K that follows it on its stream
-      const int ahead = w.step;
-      for (int i = 0; i < min(ahead, w.n); ++i) load(&tm_k, w.it.tile0 + i, false);
+      // The order in which the tiles are used: V of a tile right in front of the K that follows it on its stream.  The query
+      // rows come behind the first four tiles, which do not wait for the item in front to end.
+      const int ahead = w.step, total = 2 * w.n;
+      int issued = 0;
+      auto step = [&](const CUtensorMap *tm, int j, bool is_v) {
+        if (issued == min(4, total - 1)) load_q();
+        ++issued;
+        load(tm, j, is_v);
+      };
+      for (int i = 0; i < min(ahead, w.n); ++i) step(&tm_k, w.it.tile0 + i, false);
       for (int i = 0; i < w.n; ++i) {
-        load(&tm_v, w.it.tile0 + i, true);
-        if (i + ahead < w.n) load(&tm_k, w.it.tile0 + i + ahead, false);
+        step(&tm_v, w.it.tile0 + i, true);
+        if (i + ahead < w.n) step(&tm_k, w.it.tile0 + i + ahead, false);
       }
     }
   } else if (warp == 1) {
@@ -305,7 +358,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     const uint64_t dk = smem_desc(smem_u32(smem + C::kOffKv)), dv = smem_desc(smem_u32(smem + C::kOffKv), C::kSub);
     const uint32_t b_full = smem_u32(kv_full), b_empty = smem_u32(kv_empty), b_s = smem_u32(s_full), b_p = smem_u32(p_full),
                    b_o = smem_u32(o_full), b_q = smem_u32(q_empty);
-    uint32_t st = 0, st_par = 0, q_par = 0, p_par0 = 0, p_par1 = 0;
+    uint32_t st = 0, st_par = 0, k_item = 0, p_par0 = 0, p_par1 = 0;
     auto take = [&]() {  // the next stage of the ring, filled
       const uint32_t now = st;
       wait(b_full + now * 8, st_par);
@@ -334,11 +387,11 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       par ^= 1;
       tc_fence_after();
     };
-    for (int r = 0, item = item_of(0); item < p.items; item = item_of(++r)) {
-      const Work w = make_work(seqs, p, item);
+    for (Items it = items; it.item >= 0; it.item = it.next(wait, lane) ? it.item : -1) {
+      const Work w = make_work(seqs, p, it.item);
       if (w.n == 0) continue;
-      wait(q_full, q_par);
-      q_par ^= 1;
+      wait(k_item & 1 ? q_full2 : q_full, (k_item >> 1) & 1);
+      ++k_item;
       if (w.dual) {
         // V of tile j, then K of tile j + 1; the streams alternate.  The next pair of stages is waited for behind stream 0's
         // products, while they run.
@@ -407,6 +460,30 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     if (elect_one()) tc_commit(fin);  // every arrival that the instructions still owe has happened before the block ends
     __syncwarp();
     wait(fin, 0);
+  } else if (warp == 3) {
+    // ------------------------------------------------------------------ the next items
+    for (uint32_t n = 0;; ++n) {
+      const uint32_t slot = n & 1;
+      if (n >= 2) wait(&clc_empty[slot], ((n >> 1) - 1) & 1);
+      if (*abort_flag) break;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&clc_full[slot], 16);
+        asm volatile(
+            "clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                items.resp + slot * 16),
+            "r"(smem_u32(&clc_full[slot]))
+            : "memory");
+      }
+      wait(&clc_full[slot], (n >> 1) & 1);
+      uint32_t ok;
+      asm volatile(
+          "{\n\t.reg .pred p;\n\t.reg .b128 h;\n\tld.shared.b128 h, [%1];\n\t"
+          "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+          : "=r"(ok)
+          : "r"(items.resp + slot * 16)
+          : "memory");
+      if (ok == 0) break;  // nothing left (asking again would not be allowed)
+    }
   } else if (warp < C::kFirstSoft) {
     if constexpr (KV8) {
       if (warp >= 4) {
@@ -414,8 +491,8 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       // A byte u = x + 128 under 0x64 is the fp16 1024 + u, exactly; 1152 taken off gives x.
       uint32_t c = 0;
       const int r_first = (warp - 4) * (kTile / 4);
-      for (int r = 0, item = item_of(0); item < p.items; item = item_of(++r)) {
-        const Work w = make_work(seqs, p, item);
+      for (Items it = items; it.item >= 0; it.item = it.next(wait, lane) ? it.item : -1) {
+        const Work w = make_work(seqs, p, it.item);
         if (w.n == 0) continue;
         const ChunkSeq &e = seqs.s[w.it.seq];
         const int alive0 = p.window > 0 ? max(0, e.ctx - e.q_len - p.window + 1) : 0, alive1 = e.ctx;
@@ -488,14 +565,24 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     const int row = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)(warp & 3) * 32 << 16;
     const uint32_t t_s = tmem + lanes + s * kTile + hf * 64, t_o = tmem + lanes + C::kColO + s * D + hf * (D / 2);
-    const int pair = 1 + s * 4 + (warp & 3);  // named barrier of the two warps of these rows
+    // Barriers of the two warps of these rows, and of all softmax warps: waits like the others, bounded
+    const uint32_t b_pair = smem_u32(&pair_bars[s * 4 + (warp & 3)]), b_merge = smem_u32(merge_bar);
+    uint32_t pair_par = 0, merge_par = 0;
+    auto sync_on = [&](uint32_t bar, uint32_t &par) {
+      __syncwarp();
+      if (lane == 0) mbar_arrive_at(bar);
+      wait(bar, par);
+      par ^= 1;
+    };
+    auto pair_sync = [&]() { sync_on(b_pair, pair_par); };
+    auto merge_sync = [&]() { sync_on(b_merge, merge_par); };
     float *x_mine = xch + (s * 2 + hf) * kRows + row, *x_other = xch + (s * 2 + (hf ^ 1)) * kRows + row;
     const int g = p.group;
     const int tok_in = row / g, head_in = row - tok_in * g;
-    const bool speaker = s == 1 && hf == 0 && (warp & 3) == 0;  // the warp that frees Q's space for its stream
-    uint32_t s_round = 0, o_round = 0, q_round = 0;
-    for (int r = 0, item = item_of(0); item < p.items; item = item_of(++r)) {
-      const Work w = make_work(seqs, p, item);
+    const bool speaker = s == 1 && hf == 0 && (warp & 3) == 0;  // the warp that speaks for its stream
+    uint32_t s_round = 0, o_round = 0, k_items = 0;
+    for (Items it = items; it.item >= 0; it.item = it.next(wait, lane) ? it.item : -1) {
+      const Work w = make_work(seqs, p, it.item);
       const ChunkSeq &e = seqs.s[w.it.seq];
       const int tok0 = w.dual && s == 1 ? w.t1 : w.it.tok0;
       const int ntok = min(half, w.it.tok1 - tok0);
@@ -504,6 +591,8 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       const int pos0 = e.ctx - e.q_len + tok0;
       const int pos = live ? pos0 + tok_in : -1;
       const int j_beg = s == 0 ? w.j0[0] : w.j0[1], j_end = s == 0 ? w.j1[0] : w.j1[1];
+      const uint32_t k_item = k_items;
+      if (w.n > 0) ++k_items;
       float m = -INFINITY, l = 0.f;
       float sc = p.scale_log2e;  // score -> log2 domain
       float shift = 0.f;         // int8 with offsets: the part of a row's scores that all tokens share (for the lse)
@@ -530,14 +619,14 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
             }
           }
           *x_mine = top;
-          named_bar_sync(pair, 64);
+          pair_sync();
           top = fmaxf(top, *x_other);
-          named_bar_sync(pair, 64);
+          pair_sync();
           if (of != nullptr) {
             *x_mine = off;
-            named_bar_sync(pair, 64);
+            pair_sync();
             off += *x_other;
-            named_bar_sync(pair, 64);
+            pair_sync();
           }
           const int ex = min(max((int)(__float_as_uint(top) >> 23) - 127, -113), 128);  // exponent of the largest
           const float up = top > 0.f ? __uint_as_float((uint32_t)(127 + 13 - ex) << 23) : 1.f;
@@ -555,17 +644,16 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           fence_proxy_async();
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(q_full);
-        wait(q_full, q_round & 1);  // (single: stream 1 takes its rows' scales from stream 0; and nobody runs ahead)
-        ++q_round;
+        uint64_t *bar = k_item & 1 ? q_full2 : q_full;
+        if (lane == 0) mbar_arrive(bar);
+        wait(bar, (k_item >> 1) & 1);  // (single: stream 1 takes its rows' scales from stream 0; and nobody runs ahead)
         if (!w.dual && s == 1) sc = q_scale[row];
       }
       if (!KV8 && speaker && w.n > 0) {
-        // One of the two arrivals that free Q's space is stream 1's: at once (dual), or when the merge is through with it
-        // (single).  It comes behind the arrival of the item's rows, so never before the one of the item in front.
-        wait(q_full, q_round & 1);
-        ++q_round;
-        if (w.dual && lane == 0) mbar_arrive(q_empty);
+        // Stream 1 says when the second tile of Q's space is not (dual), or not any more (single: behind the merge), a merge
+        // buffer.  It does so behind the arrival of the item's rows, so never before the item in front is done with.
+        wait(k_item & 1 ? q_full2 : q_full, (k_item >> 1) & 1);
+        if (w.dual && lane == 0) mbar_arrive(&m_free[k_item & 1]);
       }
       for (int j = j_beg; j < j_end; j += w.step) {
         wait(&s_full[s], s_round & 1);
@@ -598,7 +686,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
           // (the next tile's exchange comes behind that tile's s_full, which both warps' p_full of this one precede)
           *x_mine = mx;
-          named_bar_sync(pair, 64);
+          pair_sync();
           mx = fmaxf(mx, *x_other) * sc;
           const bool first = j == j_beg;
           const bool grow = mx > m + kSlack;  // also for the first value: m is -inf
@@ -662,17 +750,17 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       // the row's sum (o_full: both warps are through with the exchanges of the tiles)
       if (warp_live) {
         *x_mine = l;
-        named_bar_sync(pair, 64);
+        pair_sync();
         l += *x_other;
       }
       const bool two = !w.dual && w.n > 1;  // two states of the same rows
       float scale0 = 1.f, scale1 = 0.f, m_out = m, l_out = l;
       if (two) {
         if (s == 1) {
-          if (warp_live) named_bar_sync(pair, 64);  // the sums have been read
+          if (warp_live) pair_sync();  // the sums have been read
           *x_mine = hf == 0 ? m : l;
         }
-        named_bar_sync(9, 512);
+        merge_sync();
         if (s == 0) {
           const float m1 = xch[2 * kRows + row], l1 = xch[3 * kRows + row];
           m_out = fmaxf(m, m1);
@@ -712,7 +800,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
               for (int i = 0; i < 16; ++i) buf[(c + i) * kRows] = __uint_as_float(o[i]);
               if (c + 16 < kPart) continue;
             }
-            if (c == (s == 1 ? kPart - 16 : 0)) named_bar_sync(9, 512);
+            if (c == (s == 1 ? kPart - 16 : 0)) merge_sync();
             if (s == 1) continue;
 #pragma unroll
             for (int i = 0; i < 16; ++i)
@@ -741,18 +829,18 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         }
         if (two) {
           fence_proxy_async();  // the buffer's next use is by the loads
-          named_bar_sync(10, 512);
+          merge_sync();
         }
       }
       // the merge buffer lies over Q's second tile: only now may the next item's rows come in
-      if (!KV8 && speaker && w.n > 0 && !w.dual && lane == 0) mbar_arrive(q_empty);
+      if (!KV8 && speaker && w.n > 0 && !w.dual && lane == 0) mbar_arrive(&m_free[k_item & 1]);
       if (writes && hf == 0) {
         m_out += shift;
         if (split) *reinterpret_cast<float2 *>(p.part_ml + prow * 2) = make_float2(m_out, l_out);
         else if (p.lse != nullptr) p.lse[orow] = l_out > 0.f ? (m_out + log2f(l_out)) * kLn2 : -INFINITY;
       }
       // the sums have been read before the next item's exchanges
-      if (warp_live && !two) named_bar_sync(pair, 64);
+      if (warp_live && !two) pair_sync();
       tc_fence_before();  // the reads of O are ordered before the next item's products (which wait for its P)
     }
   }
@@ -849,7 +937,7 @@ int encode(CUtensorMap *tm, const void *base, int32_t dtype, bool swizzle, const
 }
 
 template <typename T, int D, bool KV8, int N>
-int launch_sized(const MscoChunkDesc &d, const ChunkParams &p, const ChunkSeq *src, int64_t q_rows, int sms,
+int launch_sized(const MscoChunkDesc &d, const ChunkParams &p, const ChunkSeq *src, int64_t q_rows,
                  cudaStream_t stream) {
   using C = Cfg<D, KV8>;
   static_assert(C::kSmem <= 232448, "shared memory of one SM exceeded");
@@ -882,7 +970,7 @@ int launch_sized(const MscoChunkDesc &d, const ChunkParams &p, const ChunkSeq *s
   auto kfn = chunk_tc_kernel<T, D, KV8, N>;
   // set per call: the attribute belongs to a device
   MSCO_CUDA_CHECK(cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
-  kfn<<<std::min(p.items, sms), C::kThreads, C::kSmem, stream>>>(tq, tk, tv, p, seqs);
+  kfn<<<p.items, C::kThreads, C::kSmem, stream>>>(tq, tk, tv, p, seqs);
   MSCO_CUDA_CHECK(cudaGetLastError());
   if (split) {
     cudaLaunchConfig_t cfg = {};
@@ -900,20 +988,20 @@ int launch_sized(const MscoChunkDesc &d, const ChunkParams &p, const ChunkSeq *s
 }
 
 template <typename T, int D, bool KV8>
-int launch_typed(const MscoChunkDesc &d, const ChunkParams &p, const ChunkSeq *src, int64_t q_rows, int sms,
+int launch_typed(const MscoChunkDesc &d, const ChunkParams &p, const ChunkSeq *src, int64_t q_rows,
                  cudaStream_t stream) {
-  if (p.nseq <= kChunkSeqsSmall) return launch_sized<T, D, KV8, kChunkSeqsSmall>(d, p, src, q_rows, sms, stream);
-  return launch_sized<T, D, KV8, kChunkSeqsMax>(d, p, src, q_rows, sms, stream);
+  if (p.nseq <= kChunkSeqsSmall) return launch_sized<T, D, KV8, kChunkSeqsSmall>(d, p, src, q_rows, stream);
+  return launch_sized<T, D, KV8, kChunkSeqsMax>(d, p, src, q_rows, stream);
 }
 
 template <typename T>
-int launch_of(const MscoChunkDesc &d, const ChunkParams &p, const ChunkSeq *src, int64_t q_rows, int sms, cudaStream_t stream) {
+int launch_of(const MscoChunkDesc &d, const ChunkParams &p, const ChunkSeq *src, int64_t q_rows, cudaStream_t stream) {
   const bool i8 = d.kv_dtype == MSCO_DTYPE_I8;
   if (d.head_dim == 64)
-    return i8 ? launch_typed<T, 64, true>(d, p, src, q_rows, sms, stream)
-              : launch_typed<T, 64, false>(d, p, src, q_rows, sms, stream);
-  return i8 ? launch_typed<T, 128, true>(d, p, src, q_rows, sms, stream)
-            : launch_typed<T, 128, false>(d, p, src, q_rows, sms, stream);
+    return i8 ? launch_typed<T, 64, true>(d, p, src, q_rows, stream)
+              : launch_typed<T, 64, false>(d, p, src, q_rows, stream);
+  return i8 ? launch_typed<T, 128, true>(d, p, src, q_rows, stream)
+            : launch_typed<T, 128, false>(d, p, src, q_rows, stream);
 }
 
 }  // namespace
@@ -927,10 +1015,10 @@ bool chunk_tc_supported(const MscoChunkDesc &d) {
          d.num_blocks * (int64_t)bs < (1ll << 31) && d.num_blocks * (int64_t)d.num_kv_heads < (1ll << 31);
 }
 
-int launch_chunk_tc(const MscoChunkDesc &d, const ChunkParams &p, const ChunkSeq *seqs, int64_t q_rows, int sms,
+int launch_chunk_tc(const MscoChunkDesc &d, const ChunkParams &p, const ChunkSeq *seqs, int64_t q_rows,
                     cudaStream_t stream) {
-  return d.q_dtype == MSCO_DTYPE_F16 ? launch_of<__half>(d, p, seqs, q_rows, sms, stream)
-                                     : launch_of<__nv_bfloat16>(d, p, seqs, q_rows, sms, stream);
+  return d.q_dtype == MSCO_DTYPE_F16 ? launch_of<__half>(d, p, seqs, q_rows, stream)
+                                     : launch_of<__nv_bfloat16>(d, p, seqs, q_rows, stream);
 }
 
 int chunk_tc_status() {
