@@ -54,9 +54,10 @@ struct Cfg {
   static constexpr int kOffKv = 2 * kQBytes;
   static constexpr int kOffRaw = kOffKv + kStages * kStageBytes;
   static constexpr int kOffBar = kOffRaw + kRaw * kRawBytes;
-  static constexpr int kNumBars = 2 * kStages + 2 * kRaw + 26;
+  static constexpr int kNumBars = 2 * kStages + 2 * kRaw + 18;
   static constexpr int kOffResp = (kOffBar + kNumBars * 8 + 16 + 15) / 16 * 16;  // answers of the launch control
-  static constexpr int kOffXch = kOffResp + 32;  // [stream][half][row]: what the two threads of a row exchange
+  static constexpr int kOffPair = kOffResp + 32;               // [8] items of the softmax pairs
+  static constexpr int kOffXch = kOffPair + 32;  // [stream][half][row]: what the two threads of a row exchange
   static constexpr int kSmem = kOffXch + 2 * 2 * kRows * 4 + (KV8 ? kRows * 4 : 0);
   // Of eight pairs of probabilities, those whose exponentials the FMA pipe computes.  At head_dim 128 the special-function
   // unit alone (1024 clocks a tile and stream) is as long as the two products: 2 of 8 took the prompt of 8192 tokens from
@@ -190,7 +191,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   uint64_t *kv_full = bars, *kv_empty = bars + C::kStages;
   uint64_t *q_full = bars + 2 * C::kStages, *q_empty = q_full + 1, *s_full = q_full + 2, *p_full = q_full + 4,
            *o_full = q_full + 6, *tail = q_full + 8, *fin = q_full + 9, *clc_full = q_full + 10, *clc_empty = q_full + 12,
-           *m_free = q_full + 14, *pair_bars = q_full + 16, *merge_bar = q_full + 24, *q_full2 = q_full + 25, *raw_full = q_full + 26, *raw_empty = raw_full + C::kRaw;
+           *m_free = q_full + 14, *merge_bar = q_full + 16, *q_full2 = q_full + 17, *raw_full = q_full + 18, *raw_empty = raw_full + C::kRaw;
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + C::kNumBars);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
   float *xch = reinterpret_cast<float *>(smem + C::kOffXch);
@@ -215,11 +216,10 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       mbar_init(&o_full[s], 1);
     }
     mbar_init(tail, 1);
-    for (int i = 0; i < 8; ++i) mbar_init(&pair_bars[i], 2);
     mbar_init(merge_bar, 2 * kSoftWarps);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&clc_full[i], 1);
-      mbar_init(&clc_empty[i], 2 + 16 + (KV8 ? 4 : 0));  // loads, matrix instructions, softmax, conversion
+      mbar_init(&clc_empty[i], 2 + kSoftWarps + (KV8 ? 4 : 0));  // loads, matrix instructions, a warp of each softmax pair, conversion
       mbar_init(&m_free[i], 1);
     }
     mbar_init(fin, 1);
@@ -565,24 +565,28 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     const int row = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)(warp & 3) * 32 << 16;
     const uint32_t t_s = tmem + lanes + s * kTile + hf * 64, t_o = tmem + lanes + C::kColO + s * D + hf * (D / 2);
-    // Barriers of the two warps of these rows, and of all softmax warps: waits like the others, bounded
-    const uint32_t b_pair = smem_u32(&pair_bars[s * 4 + (warp & 3)]), b_merge = smem_u32(merge_bar);
-    uint32_t pair_par = 0, merge_par = 0;
-    auto sync_on = [&](uint32_t bar, uint32_t &par) {
+    // Named barrier of the two warps of these rows.  One of them takes the items for both, so that neither leaves (when a
+    // wait has run out, too) while the other still comes to this barrier.  The barrier of all softmax warps, once in an item
+    // that merges, is a bounded wait like the others: pairs may leave on their own.
+    const int pair = 1 + s * 4 + (warp & 3);
+    volatile int *pair_item = reinterpret_cast<volatile int *>(smem + C::kOffPair) + s * 4 + (warp & 3);
+    const uint32_t b_merge = smem_u32(merge_bar);
+    uint32_t merge_par = 0;
+    auto pair_sync = [&]() { named_bar_sync(pair, 64); };
+    auto merge_sync = [&]() {
       __syncwarp();
-      if (lane == 0) mbar_arrive_at(bar);
-      wait(bar, par);
-      par ^= 1;
+      if (lane == 0) mbar_arrive_at(b_merge);
+      wait(b_merge, merge_par);
+      merge_par ^= 1;
     };
-    auto pair_sync = [&]() { sync_on(b_pair, pair_par); };
-    auto merge_sync = [&]() { sync_on(b_merge, merge_par); };
     float *x_mine = xch + (s * 2 + hf) * kRows + row, *x_other = xch + (s * 2 + (hf ^ 1)) * kRows + row;
     const int g = p.group;
     const int tok_in = row / g, head_in = row - tok_in * g;
     const bool speaker = s == 1 && hf == 0 && (warp & 3) == 0;  // the warp that speaks for its stream
     uint32_t s_round = 0, o_round = 0, k_items = 0;
-    for (Items it = items; it.item >= 0; it.item = it.next(wait, lane) ? it.item : -1) {
-      const Work w = make_work(seqs, p, it.item);
+    Items it = items;
+    for (int item = it.item; item >= 0;) {
+      const Work w = make_work(seqs, p, item);
       const ChunkSeq &e = seqs.s[w.it.seq];
       const int tok0 = w.dual && s == 1 ? w.t1 : w.it.tok0;
       const int ntok = min(half, w.it.tok1 - tok0);
@@ -839,9 +843,14 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         if (split) *reinterpret_cast<float2 *>(p.part_ml + prow * 2) = make_float2(m_out, l_out);
         else if (p.lse != nullptr) p.lse[orow] = l_out > 0.f ? (m_out + log2f(l_out)) * kLn2 : -INFINITY;
       }
-      // the sums have been read before the next item's exchanges
-      if (warp_live && !two) pair_sync();
       tc_fence_before();  // the reads of O are ordered before the next item's products (which wait for its P)
+      if (hf == 0) {
+        const bool more = it.next(wait, lane);
+        if (lane == 0) *pair_item = more ? it.item : -1;
+      }
+      pair_sync();
+      item = *pair_item;
+      pair_sync();
     }
   }
   tc_fence_before();
