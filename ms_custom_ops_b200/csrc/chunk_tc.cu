@@ -783,12 +783,15 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
                            (tok0 - w.it.tok0) * g + row;
       const float inv = split ? 1.f : (l_out > 0.f ? 1.f / l_out : 0.f);
       const bool writes = live && (w.dual || s == 0);
-      constexpr int kPart = D / 4;  // this half's columns that go through the merge buffer (the space of Q's second tile) at a time
-      float *buf = reinterpret_cast<float *>(smem + C::kQBytes) + hf * (kPart * kRows) + row;
+      // This half's columns that go through the merge buffer (the space of Q's second tile) at a time: with up to 64 rows
+      // all of them.
+      const bool few = ntok * g <= 64;
+      const int part = few ? D / 2 : D / 4, stride = few ? 64 : kRows;
+      float *buf = reinterpret_cast<float *>(smem + C::kQBytes) + hf * (part * stride) + row;
 #pragma unroll 1
-      for (int c0 = 0; c0 < D / 2; c0 += kPart) {
+      for (int c0 = 0; c0 < D / 2; c0 += part) {
 #pragma unroll 1
-        for (int c = 0; c < kPart; c += 16) {
+        for (int c = 0; c < part; c += 16) {
           uint32_t o[16];
           if (warp_live && has) {
             tmem_ld16(t_o + c0 + c, o);
@@ -801,14 +804,15 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
             // stream 1 lays its columns down one by one (consecutive rows: no bank conflicts), stream 0 adds them in
             if (s == 1) {
 #pragma unroll
-              for (int i = 0; i < 16; ++i) buf[(c + i) * kRows] = __uint_as_float(o[i]);
-              if (c + 16 < kPart) continue;
+              for (int i = 0; i < 16; ++i)
+                if (warp_live) buf[(c + i) * stride] = __uint_as_float(o[i]);
+              if (c + 16 < part) continue;
             }
-            if (c == (s == 1 ? kPart - 16 : 0)) merge_sync();
+            if (c == (s == 1 ? part - 16 : 0)) merge_sync();
             if (s == 1) continue;
 #pragma unroll
             for (int i = 0; i < 16; ++i)
-              o[i] = __float_as_uint(__uint_as_float(o[i]) * scale0 + buf[(c + i) * kRows] * scale1);
+              o[i] = __float_as_uint(__uint_as_float(o[i]) * scale0 + (warp_live ? buf[(c + i) * stride] : 0.f) * scale1);
           }
           if (writes) {
             const int col = hf * (D / 2) + c0 + c;

@@ -22,7 +22,7 @@ namespace cg = cooperative_groups;
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kMaxCluster = 8;
+constexpr int kMaxCluster = 8;  // (at most 64 warps: two sums per lane)
 
 struct VerifyArgs {
   const void *target, *draft;
@@ -38,11 +38,11 @@ __device__ __forceinline__ double weight_of(float p, float q) {
   return w > 0.0 ? w : 0.0;
 }
 
-constexpr int kLane = 16;            // vocabulary entries per lane and chunk
+constexpr int kLane = 8;             // vocabulary entries per lane and chunk
 constexpr int kChunk = 32 * kLane;   // entries of a chunk
 
-// Entries t0 .. t0 + 511 of a row, 16 per lane, 0 behind the end.  VEC: rows are 16-byte aligned (and t0 is a multiple of
-// 512), so a lane's entries come in 16-byte pieces, piece i of all lanes adjacent; otherwise one entry at a time.
+// Entries t0 .. t0 + 255 of a row, 8 per lane, 0 behind the end.  VEC: rows are 16-byte aligned (and t0 is a multiple of
+// 256), so a lane's entries come in 16-byte pieces, piece i of all lanes adjacent; otherwise one entry at a time.
 // The entry `skip` reads as 0.
 template <typename T, bool VEC>
 __device__ __forceinline__ void load_chunk(const T *row, int t0, int end, int lane, int skip, float (&x)[kLane]) {
@@ -70,12 +70,12 @@ __device__ __forceinline__ void load_chunk(const T *row, int t0, int end, int la
 }
 
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(kThreads) verify_kernel(VerifyArgs a) {
+__global__ void __launch_bounds__(kThreads, 4) verify_kernel(VerifyArgs a) {
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = (int)cluster.block_rank(), ranks = (int)cluster.num_blocks();
   const int b = blockIdx.x / ranks;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  __shared__ double sums[kWarps];
+  __shared__ double all_sums[2][kWarps];  // per mode
   const T *target = static_cast<const T *>(a.target) + (int64_t)b * (a.drafts + 1) * a.vocab;
   const T *draft = static_cast<const T *>(a.draft);
   if (draft != nullptr) draft += (int64_t)b * a.drafts * a.vocab;
@@ -134,22 +134,35 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(VerifyArgs a) {
       if (lane == k) mine = sum;
       s += sum;
     }
+    double *sums = all_sums[mode];
     if (lane == 0) sums[warp] = s;
     cluster.sync();
-    double total = 0.0, before = 0.0;
-    for (int r = 0; r < ranks; ++r) {
-      const double *rs = cluster.map_shared_rank(sums, r);
+    // every warp scans all sums in the same way, so all agree on the total and on whose part holds the border
+    double part[2], own[2];
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        if (r * kWarps + w == id) before = total;
-        total += rs[w];
+    for (int k = 0; k < 2; ++k) {
+      const int w = k * 32 + lane;
+      own[k] = part[k] = w < warps ? cluster.map_shared_rank(sums, w / kWarps)[w % kWarps] : 0.0;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const double up = __shfl_up_sync(0xffffffffu, part[k], o);
+        if (lane >= o) part[k] += up;
       }
     }
-    // every warp adds the sums in the same order, so all agree on the total and on whose part holds the border
+    part[1] += __shfl_sync(0xffffffffu, part[0], 31);
+    const double total = __shfl_sync(0xffffffffu, part[1], 31);
     const double goal = (double)__ldg(u + a.drafts) * total;
     found = goal >= 0.0 && goal < total;  // not for a row that is nowhere positive, nor for uniform outside [0, 1)
-    here = found && before <= goal && before + s > goal;
-    cluster.sync();  // the sums have been read
+    // the first part that counts whose running sum passes the goal (should the last place of the sums leave none, the last
+    // part that counts)
+    const uint64_t counts = (uint64_t)__ballot_sync(0xffffffffu, own[1] > 0.0) << 32 | __ballot_sync(0xffffffffu, own[0] > 0.0);
+    const uint64_t over = counts & ((uint64_t)__ballot_sync(0xffffffffu, part[1] > goal) << 32 |
+                                    __ballot_sync(0xffffffffu, part[0] > goal));
+    const int owner = over != 0 ? __ffsll((long long)over) - 1 : 63 - __clzll((long long)counts);
+    here = found && owner == id;
+    const int prev = max(owner - 1, 0);
+    const double prev0 = __shfl_sync(0xffffffffu, part[0], prev & 31), prev1 = __shfl_sync(0xffffffffu, part[1], prev & 31);
+    const double before = owner == 0 ? 0.0 : (prev < 32 ? prev0 : prev1);
     if (!(total > 0.0)) continue;
     if (here) {
       // the chunk in which the running sum passes the goal, then the entry
@@ -159,9 +172,8 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(VerifyArgs a) {
         const double up = __shfl_up_sync(0xffffffffu, c, o);
         if (lane >= o) c += up;
       }
-      const unsigned over = __ballot_sync(0xffffffffu, before + c > goal);
-      // (sums taken in another order differ in the last place: the last chunk that counts then)
       const unsigned some = __ballot_sync(0xffffffffu, mine > 0.0);
+      const unsigned over = some & __ballot_sync(0xffffffffu, before + c > goal);
       const int k = over != 0 ? __ffs(over) - 1 : 31 - __clz(some);
       double run = before + (__shfl_sync(0xffffffffu, c, k) - __shfl_sync(0xffffffffu, mine, k));
       int last = -1;
@@ -199,6 +211,7 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(VerifyArgs a) {
     }
     break;
   }
+  cluster.barrier_arrive();  // this block reads no other's sums any more
   int32_t *out = a.tokens + (int64_t)b * (a.drafts + 1);
   if (here && lane == 0) out[n] = drawn;
   if (rank == 0 && warp == 0) {
@@ -206,6 +219,7 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(VerifyArgs a) {
     for (int i = lane; i <= a.drafts; i += 32)
       if (i != n || !found) out[i] = i < n ? __ldg(dtok + i) : -1;
   }
+  cluster.barrier_wait();    // and none reads this block's
 }
 
 template <typename T>

@@ -110,84 +110,138 @@ __device__ __forceinline__ void unpack8(const uint4 &v, float (&x)[8]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] = to_f32(e[i]);
 }
-__device__ __forceinline__ uint4 load_stream(const void *p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
-}
-
-// head_dim 64 / 128 / 256, 16-byte rows.  D / 8 lanes own a head row, eight consecutive elements each; such a group takes
-// ROWS consecutive head rows of one token, so the cosines and sines are fetched once for them and all ROWS loads are in
-// flight before the first is used.  The other element of a pair is in the same lane (interleaved) or rotary / 16 lanes on.
-template <typename T, int D, bool I8, bool INTER, bool NORM, int ROWS>
+// head_dim 64 / 128 / 256, 16-byte rows.  D / 8 lanes own a head row; such a group takes ROWS consecutive head rows of one
+// token, all queries, all keys or all values (ROWS divides both head counts), so that the cosines, sines and weights are
+// fetched once for them and all loads are in flight before the first is used.  A lane has eight consecutive elements
+// (interleaved: both of each pair); when whole heads are rotated by halves (SPLIT) it has four of each half instead, so
+// that no pair lies in two lanes -- otherwise the other element comes from rotary / 16 lanes on.
+// Bound by issue slots and shuffles before memory: with eight consecutive elements, one shuffle per element and a choice
+// of source per row the prefill step of 16384 tokens took 110 to 130 us.
+template <typename T, int D, bool I8, bool INTER, bool NORM, bool SPLIT, int ROWS>
 __global__ void __launch_bounds__(256) rope_cache_vec_kernel(RopeArgs a) {
   constexpr int L = D / 8;
-  const int sub = threadIdx.x & (L - 1);
-  const int rows = a.q_heads + 2 * a.kv_heads;
-  const int chunks = (rows + ROWS - 1) / ROWS;
-  const int64_t group = ((int64_t)blockIdx.x * 256 + threadIdx.x) / L;
-  const int64_t t_raw = group / chunks;
-  const bool in = t_raw < a.tokens;  // lanes behind the last token go along (shuffles), and store nothing
-  const int64_t t = in ? t_raw : a.tokens - 1;
-  const int r0 = (int)(group - t_raw * chunks) * ROWS;
-  const int d0 = sub * 8;
+  const int lane = threadIdx.x & 31, sub = threadIdx.x & (L - 1);
+  const unsigned mask = L == 32 ? 0xffffffffu : ((1u << (L & 31)) - 1) << (lane & ~(L - 1));
+  const int q_chunks = a.q_heads / ROWS, kv_chunks = a.kv_heads / ROWS, chunks = q_chunks + 2 * kv_chunks;
+  const uint32_t group = blockIdx.x * (256 / L) + threadIdx.x / L;  // (fewer than 2^32: the launch checks)
+  const uint32_t t = group / (uint32_t)chunks;
+  if (t >= a.tokens) return;  // whole groups: the shuffles below stay inside one
+  const int ch = (int)(group - t * chunks);
+  const int kind = ch < q_chunks ? 0 : (ch < q_chunks + kv_chunks ? 1 : 2);
+  const int h0 = (kind == 0 ? ch : (kind == 1 ? ch - q_chunks : ch - q_chunks - kv_chunks)) * ROWS;
+  const int d0 = SPLIT ? sub * 4 : sub * 8, d1 = SPLIT ? D / 2 + sub * 4 : d0 + 4;  // first of the lane's two quads
+  const T *src = static_cast<const T *>(kind == 0 ? a.q : (kind == 1 ? a.k : a.v)) +
+                 (int64_t)t * (kind == 0 ? a.q_stride : (kind == 1 ? a.k_stride : a.v_stride)) + h0 * D;
   uint4 raw[ROWS];
 #pragma unroll
   for (int i = 0; i < ROWS; ++i) {
-    const int r = min(r0 + i, rows - 1);
-    const T *src = r < a.q_heads ? static_cast<const T *>(a.q) + t * a.q_stride + (int64_t)r * D
-                   : r < a.q_heads + a.kv_heads
-                       ? static_cast<const T *>(a.k) + t * a.k_stride + (int64_t)(r - a.q_heads) * D
-                       : static_cast<const T *>(a.v) + t * a.v_stride + (int64_t)(r - a.q_heads - a.kv_heads) * D;
-    raw[i] = load_stream(src + d0);
-  }
-  const int32_t pos = __ldg(a.positions + t);
-  const int64_t slot = __ldg(a.slots + t);
-  const bool pos_ok = pos >= 0 && pos < a.max_positions;
-  const bool store = slot >= 0 && slot < a.slots_total && pos_ok;
-  if (in && r0 == 0 && sub == 0 && a.oob != nullptr && (!pos_ok || slot >= a.slots_total)) atomicAdd(a.oob, 1);
-  const int half = a.rotary >> 1;
-  const bool turns = d0 < a.rotary;
-  const bool first = INTER || d0 < half;
-  float c[8], sn[8];  // INTER: four pairs
-  {
-    const float *cs = a.cos_sin + (int64_t)(pos_ok ? pos : 0) * a.rotary;
-    const int i0 = INTER ? d0 >> 1 : (first ? d0 : d0 - half);
-    constexpr int kN = INTER ? 4 : 8;
-#pragma unroll
-    for (int i = 0; i < kN; i += 4) {
-      const float4 cc = turns && pos_ok ? __ldg(reinterpret_cast<const float4 *>(cs + i0 + i)) : make_float4(1, 1, 1, 1);
-      c[i] = cc.x; c[i + 1] = cc.y; c[i + 2] = cc.z; c[i + 3] = cc.w;
-      const float4 ss = turns && pos_ok ? __ldg(reinterpret_cast<const float4 *>(cs + half + i0 + i)) : make_float4(0, 0, 0, 0);
-      sn[i] = ss.x; sn[i + 1] = ss.y; sn[i + 2] = ss.z; sn[i + 3] = ss.w;
+    if (SPLIT) {
+      const uint2 lo = __ldg(reinterpret_cast<const uint2 *>(src + i * D + d0));
+      const uint2 hi = __ldg(reinterpret_cast<const uint2 *>(src + i * D + d1));
+      raw[i] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+    } else {
+      raw[i] = __ldg(reinterpret_cast<const uint4 *>(src + i * D + d0));
     }
   }
-  const int lane = threadIdx.x & 31;
+  const int32_t pos = __ldg(a.positions + t), slot = __ldg(a.slots + t);
+  const bool pos_ok = pos >= 0 && pos < a.max_positions;
+  const bool store = slot >= 0 && slot < a.slots_total && pos_ok;
+  if (ch == 0 && sub == 0 && a.oob != nullptr && (!pos_ok || slot >= a.slots_total)) atomicAdd(a.oob, 1);
+  if (kind != 0 && !store) return;
+  // where the rows go: consecutive rows lie `step` elements apart
+  int64_t at, step = D;
+  if (kind == 0) {
+    at = ((int64_t)t * a.q_heads + h0) * D;
+  } else if (a.layout == 1) {
+    const uint32_t blk = (uint32_t)slot / (uint32_t)a.block_size, off = (uint32_t)slot - blk * a.block_size;
+    at = (((int64_t)blk * a.kv_heads + h0) * a.block_size + off) * D;
+    step = (int64_t)a.block_size * D;
+  } else {
+    at = ((int64_t)slot * a.kv_heads + h0) * D;
+  }
+  T *dst16 = static_cast<T *>(kind == 0 ? a.q_out : (kind == 1 ? a.k_cache : a.v_cache)) + at;
+  int8_t *dst8 = static_cast<int8_t *>(kind == 1 ? a.k_cache : a.v_cache) + at;
+  const float *ds = kind == 1 ? a.k_descale : a.v_descale;
+  const int32_t *of = kind == 1 ? a.k_offset : a.v_offset;
+  auto put8 = [&](int i, const float (&y)[8]) {  // quantised row i
+    const int c = (h0 + i) * D;
+    uint32_t q8[2] = {0, 0};
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int d = k < 4 ? d0 + k : d1 + k - 4;
+      q8[k / 4] |= (uint32_t)(uint8_t)quantise(y[k], __ldg(ds + c + d), of != nullptr ? (float)__ldg(of + c + d) : 0.f)
+                   << (8 * (k & 3));
+    }
+    *reinterpret_cast<uint32_t *>(dst8 + i * step + d0) = q8[0];
+    *reinterpret_cast<uint32_t *>(dst8 + i * step + d1) = q8[1];
+  };
+  auto put16 = [&](int i, const uint4 &v) {
+    if (SPLIT) {
+      *reinterpret_cast<uint2 *>(dst16 + i * step + d0) = make_uint2(v.x, v.y);
+      *reinterpret_cast<uint2 *>(dst16 + i * step + d1) = make_uint2(v.z, v.w);
+    } else {
+      *reinterpret_cast<uint4 *>(dst16 + i * step + d0) = v;
+    }
+  };
+  if (kind == 2) {
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      if (I8) {
+        float x[8];
+        unpack8<T>(raw[i], x);
+        put8(i, x);
+      } else {
+        put16(i, raw[i]);
+      }
+    }
+    return;
+  }
+  if (kind == 0 && !pos_ok) {
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) put16(i, make_uint4(0, 0, 0, 0));
+    return;
+  }
+  const int half = a.rotary >> 1;
+  const bool turns = SPLIT || d0 < a.rotary, first = d0 < half;
+  constexpr int kN = INTER || SPLIT ? 4 : 8;  // pairs that this lane has a part in
+  float c[kN], sn[kN];
+  const float *cs = a.cos_sin + (int64_t)pos * a.rotary + (INTER ? d0 >> 1 : (SPLIT || first ? d0 : d0 - half));
+#pragma unroll
+  for (int i = 0; i < kN; i += 4) {
+    const float4 cc = turns ? __ldg(reinterpret_cast<const float4 *>(cs + i)) : make_float4(1, 1, 1, 1);
+    const float4 ss = turns ? __ldg(reinterpret_cast<const float4 *>(cs + half + i)) : make_float4(0, 0, 0, 0);
+    c[i] = cc.x; c[i + 1] = cc.y; c[i + 2] = cc.z; c[i + 3] = cc.w;
+    sn[i] = ss.x; sn[i + 1] = ss.y; sn[i + 2] = ss.z; sn[i + 3] = ss.w;
+  }
   const int other = turns ? (first ? lane + half / 8 : lane - half / 8) : lane;
+  const T *weight = static_cast<const T *>(kind == 0 ? a.q_weight : a.k_weight);
+  const bool norms = NORM && weight != nullptr;
+  float w[8];
+  if (norms) {
+    const uint2 lo = __ldg(reinterpret_cast<const uint2 *>(weight + d0)), hi = __ldg(reinterpret_cast<const uint2 *>(weight + d1));
+    unpack8<T>(make_uint4(lo.x, lo.y, hi.x, hi.y), w);
+  }
 #pragma unroll
   for (int i = 0; i < ROWS; ++i) {
-    const int r = r0 + i;
-    const int kind = r < a.q_heads ? 0 : (r < a.q_heads + a.kv_heads ? 1 : 2);
-    const int h = kind == 0 ? r : (kind == 1 ? r - a.q_heads : r - a.q_heads - a.kv_heads);
-    float x[8];
+    float x[8], y[8];
     unpack8<T>(raw[i], x);
-    if (NORM) {
+    if (norms) {
       float ss = 0.f;
 #pragma unroll
       for (int k = 0; k < 8; ++k) ss = fmaf(x[k], x[k], ss);
 #pragma unroll
-      for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      const T *weight = static_cast<const T *>(kind == 0 ? a.q_weight : a.k_weight);
-      if (kind != 2 && weight != nullptr) {
-        const float inv = 1.f / sqrtf(ss * (1.f / D) + a.eps);
-        float w[8];
-        unpack8<T>(__ldg(reinterpret_cast<const uint4 *>(weight + d0)), w);
+      for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
+      const float inv = __frsqrt_rn(ss * (1.f / D) + a.eps);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) x[k] = x[k] * inv * w[k];
-      }
+      for (int k = 0; k < 8; ++k) x[k] = x[k] * inv * w[k];
     }
-    float y[8];
-    if (INTER) {
+    if (SPLIT) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        y[k] = x[k] * c[k] - x[k + 4] * sn[k];
+        y[k + 4] = x[k + 4] * c[k] + x[k] * sn[k];
+      }
+    } else if (INTER) {
 #pragma unroll
       for (int k = 0; k < 8; k += 2) {
         y[k] = x[k] * c[k / 2] - x[k + 1] * sn[k / 2];
@@ -196,52 +250,32 @@ __global__ void __launch_bounds__(256) rope_cache_vec_kernel(RopeArgs a) {
     } else {
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        const float o = __shfl_sync(0xffffffffu, x[k], other);
-        y[k] = first ? x[k] * c[k] - o * sn[k] : x[k] * c[k] + o * sn[k];
+        const float o = __shfl_sync(mask, x[k], other);
+        y[k] = first ? x[k] * c[k % kN] - o * sn[k % kN] : x[k] * c[k % kN] + o * sn[k % kN];
       }
     }
-    if (!in || r >= rows) continue;
-    if (kind == 2) {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) y[k] = x[k];
-    }
-    const uint4 packed = make_uint4(pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3]), pack2<T>(y[4], y[5]), pack2<T>(y[6], y[7]));
-    if (kind == 0) {
-      T *dst = static_cast<T *>(a.q_out) + (t * a.q_heads + h) * D + d0;
-      *reinterpret_cast<uint4 *>(dst) = pos_ok ? packed : make_uint4(0, 0, 0, 0);
-    } else if (store) {
-      const int64_t at = cache_row(a, slot, h) + d0;
-      void *cache = kind == 1 ? a.k_cache : a.v_cache;
-      if (I8) {
-        const float *ds = (kind == 1 ? a.k_descale : a.v_descale) + h * D + d0;
-        const int32_t *of = kind == 1 ? a.k_offset : a.v_offset;
-        uint32_t q8[2] = {0, 0};
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const float off = of != nullptr ? (float)__ldg(of + h * D + d0 + k) : 0.f;
-          q8[k / 4] |= (uint32_t)(uint8_t)quantise(y[k], __ldg(ds + k), off) << (8 * (k & 3));
-        }
-        *reinterpret_cast<uint2 *>(static_cast<int8_t *>(cache) + at) = make_uint2(q8[0], q8[1]);
-      } else {
-        *reinterpret_cast<uint4 *>(static_cast<T *>(cache) + at) = kind == 2 ? raw[i] : packed;
-      }
+    if (I8 && kind == 1) {
+      put8(i, y);
+    } else {
+      put16(i, make_uint4(pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3]), pack2<T>(y[4], y[5]), pack2<T>(y[6], y[7])));
     }
   }
 }
 
-template <typename T, int D, bool I8, bool INTER, bool NORM>
+template <typename T, int D, bool I8, bool INTER, bool NORM, bool SPLIT>
 int launch_vec(const RopeArgs &a, cudaStream_t st) {
-  const int rows = a.q_heads + 2 * a.kv_heads;
   constexpr int L = D / 8;
-  auto blocks_of = [&](int per) { return (a.tokens * ((rows + per - 1) / per) * L + 255) / 256; };
-  // four rows per group once that still fills the GPU several times over, one row where latency counts
-  if (blocks_of(4) >= 148 * 8) {
-    const int64_t blocks = blocks_of(4);
-    if (blocks > 0x7fffffffLL) return fail(MSCO_ERR_INVALID_ARG, "rope_and_cache: too many rows");
-    rope_cache_vec_kernel<T, D, I8, INTER, NORM, 4><<<(unsigned)blocks, 256, 0, st>>>(a);
-  } else {
-    rope_cache_vec_kernel<T, D, I8, INTER, NORM, 1><<<(unsigned)blocks_of(1), 256, 0, st>>>(a);
-  }
+  const int rows = a.q_heads + 2 * a.kv_heads;
+  auto blocks_of = [&](int per) { return (a.tokens * (rows / per) * L + 255) / 256; };
+  if (blocks_of(1) > (int64_t)(0xffffffffu / (256 / L))) return fail(MSCO_ERR_INVALID_ARG, "rope_and_cache: too many rows");
+  // several rows per group once that still fills the GPU several times over, one row where latency counts
+  const int by = (a.q_heads | a.kv_heads) & 3;
+  if (by == 0 && blocks_of(4) >= 148 * 8)
+    rope_cache_vec_kernel<T, D, I8, INTER, NORM, SPLIT, 4><<<(unsigned)blocks_of(4), 256, 0, st>>>(a);
+  else if ((by & 1) == 0 && blocks_of(2) >= 148 * 8)
+    rope_cache_vec_kernel<T, D, I8, INTER, NORM, SPLIT, 2><<<(unsigned)blocks_of(2), 256, 0, st>>>(a);
+  else
+    rope_cache_vec_kernel<T, D, I8, INTER, NORM, SPLIT, 1><<<(unsigned)blocks_of(1), 256, 0, st>>>(a);
   MSCO_CUDA_CHECK(cudaGetLastError());
   return MSCO_OK;
 }
@@ -258,8 +292,9 @@ int launch_any(const RopeArgs &a, cudaStream_t st) {
 template <typename T, int D, bool I8>
 int launch_vec_of(const RopeArgs &a, cudaStream_t st) {
   const bool norm = a.q_weight != nullptr || a.k_weight != nullptr;
-  if (a.interleaved) return norm ? launch_vec<T, D, I8, true, true>(a, st) : launch_vec<T, D, I8, true, false>(a, st);
-  return norm ? launch_vec<T, D, I8, false, true>(a, st) : launch_vec<T, D, I8, false, false>(a, st);
+  if (a.interleaved) return norm ? launch_vec<T, D, I8, true, true, false>(a, st) : launch_vec<T, D, I8, true, false, false>(a, st);
+  if (a.rotary == D) return norm ? launch_vec<T, D, I8, false, true, true>(a, st) : launch_vec<T, D, I8, false, false, true>(a, st);
+  return norm ? launch_vec<T, D, I8, false, true, false>(a, st) : launch_vec<T, D, I8, false, false, false>(a, st);
 }
 
 // 16-byte pieces: every row address, and pairs that stay inside a lane or lie whole lanes apart
