@@ -20,7 +20,6 @@ from __future__ import annotations
 
 import ctypes as C
 import math
-import struct
 import threading
 import weakref
 
@@ -496,85 +495,31 @@ def fa_update(lse, local_out, fa_update_type=0, sp=1):
 # --------------------------------------------------------------------------
 # operators of a step with more than one token per sequence
 # --------------------------------------------------------------------------
-_DESC_STRUCT = struct.Struct(f"Pii{_host.MS_MAX_DIMS}q{_host.MS_MAX_DIMS}qii")
-assert _DESC_STRUCT.size == C.sizeof(_host.MsTensorDesc)
-_DESC_SLOTS = 24
-_PADS = tuple((0,) * (_host.MS_MAX_DIMS - n) for n in range(_host.MS_MAX_DIMS + 1))
-_torch_codes = {}  # torch.dtype -> MSCO_DTYPE_*
+def _binding():
+    """The native binding of these operators; raises if it has not been built."""
+    global _binding_module
+    if _binding_module is None:
+        _host.lib()  # the libraries first: clearer error when nothing is built
+        try:
+            from . import _torch_binding
+        except ImportError as e:
+            raise ImportError(f"{e}: build it with `python -m ms_custom_ops_b200.build`.") from e
+        _binding_module = _torch_binding
+    return _binding_module
 
 
-class _Packer:
-    """Tensor descriptors of one call, written into a buffer that the thread keeps (one struct.pack_into per
-    tensor).  Checks that all device tensors are on the first one's device."""
-
-    def __init__(self):
-        self.array = (_host.MsTensorDesc * _DESC_SLOTS)()
-        self.ptrs = [C.pointer(self.array[i]) for i in range(_DESC_SLOTS)]
-        self.size = C.sizeof(_host.MsTensorDesc)
-        self.keep = []
-        self.used = 0
-        self.device = -1
-        self.chunk_args = _host.MsChunkAttentionArgs()
-
-    def start(self, device):
-        self.used = 0
-        self.device = device
-        self.keep.clear()
-        return self
-
-    def __call__(self, t, host=False):
-        if t is None:
-            return None
-        if host and isinstance(t, (list, tuple, np.ndarray)):
-            a = np.asarray(t)
-            a = np.ascontiguousarray(a.astype(np.int32) if isinstance(t, (list, tuple)) else a)
-            self.keep.append(a)
-            values = (a.ctypes.data, _dtype_code(str(a.dtype)), a.ndim, a.shape, _contig_strides(a.shape), 1)
-        else:
-            try:
-                at = t.get_device()
-            except AttributeError:
-                raise TypeError("device tensors must be torch CUDA tensors") from None
-            if at < 0:
-                if t.numel() and not host:
-                    raise RuntimeError("the operator takes CUDA tensors (only lengths are read on the host)")
-            elif at != self.device:
-                raise RuntimeError(f"all tensors must be on one device, got cuda:{self.device} and cuda:{at}")
-            code = _torch_codes.get(t.dtype)
-            if code is None:
-                code = _torch_codes[t.dtype] = _dtype_code(t.dtype)
-            values = (t.data_ptr(), code, t.dim(), t.shape, t.stride(), 1 if at < 0 else 0)
-        ptr, code, n, shape, strides, on_host = values
-        if n > _host.MS_MAX_DIMS:
-            raise ValueError("tensors of more than 8 dimensions are not supported")
-        i = self.used
-        self.used = i + 1
-        pad = _PADS[n]
-        _DESC_STRUCT.pack_into(self.array, i * self.size, ptr, code, n, *shape, *pad, *strides, *pad, on_host, 0)
-        return self.ptrs[i]
+_binding_module = None
 
 
-def _packer(t):
-    """The thread's packer, for a call on the device of tensor `t`."""
-    try:
-        device = t.get_device()
-    except AttributeError:
-        raise TypeError("device tensors must be torch CUDA tensors") from None
-    if device < 0:
-        raise RuntimeError("the operator takes CUDA tensors (only lengths are read on the host)")
-    p = _tls.__dict__.get("packer")
-    if p is None:
-        p = _tls.packer = _Packer()
-    return p.start(device)
-
-
-def _on_device(device, call):
-    """Runs `call(stream)` with `device` current, on torch's current stream of that device."""
-    import torch
-    if torch.cuda.current_device() == device:
-        return call(torch._C._cuda_getCurrentRawStream(device))
-    with torch.cuda.device(device):
-        return call(torch._C._cuda_getCurrentRawStream(device))
+def _host_lens(t):
+    """Lengths given as a list, tuple or numpy array, as the CPU tensor that the binding reads."""
+    if isinstance(t, (list, tuple)):
+        import torch
+        return torch.tensor(t, dtype=torch.int32)
+    if isinstance(t, np.ndarray):
+        import torch
+        return torch.from_numpy(np.ascontiguousarray(t))
+    return t
 
 
 def rope_and_cache(query, key, value, key_cache, value_cache, slot_mapping, positions, cos_sin, q_weight=None,
@@ -599,16 +544,12 @@ def rope_and_cache(query, key, value, key_cache, value_cache, slot_mapping, posi
     Arithmetic in float32, rounded once.  Two tokens of a call must not have the same slot; the result must not
     share memory with the inputs (it is a new tensor).
     """
-    import torch
-    D = _packer(query)
-    out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
-    args = (D(query), D(key), D(value), D(key_cache), D(value_cache), D(slot_mapping), D(positions), D(cos_sin),
-            D(q_weight), D(k_weight), float(eps), int(bool(interleaved)), int(input_layout), D(k_descale), D(k_offset),
-            D(v_descale), D(v_offset), D(oob_count), D(out))
-    rc = _on_device(D.device, lambda stream: _host.lib().ms_custom_ops_rope_and_cache(*args, stream))
-    if rc:
-        _host.check(rc)
-    return out
+    r = _binding().rope_and_cache(query, key, value, key_cache, value_cache, slot_mapping, positions, cos_sin, q_weight,
+                                  k_weight, eps, interleaved, input_layout, k_descale, k_offset, v_descale, v_offset,
+                                  oob_count)
+    if r.__class__ is int:
+        _host.check(r)
+    return r
 
 
 def rope_and_cache_infer(query, key, value, key_cache, value_cache, slot_mapping, positions, cos_sin, q_weight=None,
@@ -625,10 +566,10 @@ def rope_and_cache_infer(query, key, value, key_cache, value_cache, slot_mapping
 
 
 def _chunk_args(a, D, query, key_cache, value_cache, block_tables, q_seq_lens, context_lens, qk_scale, window_size,
-                input_layout, k_descale, k_offset, v_descale, v_offset, oob_count, host):
+                input_layout, k_descale, k_offset, v_descale, v_offset, oob_count):
     a.query, a.key_cache, a.value_cache = D(query), D(key_cache), D(value_cache)
     a.block_tables = D(block_tables)
-    a.q_seq_lens, a.context_lens = D(q_seq_lens, **host), D(context_lens, **host)
+    a.q_seq_lens, a.context_lens = D(q_seq_lens, host_ok=True), D(context_lens, host_ok=True)
     a.k_descale, a.k_offset, a.v_descale, a.v_offset = D(k_descale), D(k_offset), D(v_descale), D(v_offset)
     a.oob_count = D(oob_count)
     a.qk_scale, a.window_size, a.input_layout = float(qk_scale), int(window_size), int(input_layout)
@@ -657,37 +598,12 @@ def chunk_attention(query, key_cache, value_cache, block_tables, q_seq_lens, con
     The i-th of q_len new tokens stands at position context_len - q_len + i; one that sees nothing gives zeros.
     The lengths are read during the call: a captured graph replays with the lengths it was captured with.
     """
-    import torch
-    D = _packer(query)
-    device, tokens = query.device, query.shape[0]
-    if out is None:
-        out = torch.empty(query.shape, dtype=query.dtype, device=device)
-        fill = True
-    else:
-        fill = False
-    lse = torch.empty(query.shape[:2], dtype=torch.float32, device=device) if return_lse else None
-    a = _chunk_args(D.chunk_args, D, query, key_cache, value_cache, block_tables, q_seq_lens, context_lens, qk_scale,
-                    window_size, input_layout, k_descale, k_offset, v_descale, v_offset, oob_count, {"host": True})
-    out_desc, lse_desc = D(out), D(lse)
-    L = _host.lib()
-    need = C.c_size_t()
-    rc = L.ms_custom_ops_chunk_attention_workspace_size(C.byref(a), C.byref(need))
-    if rc:
-        _host.check(rc)
-    # from the allocator, per call: it belongs to this call's stream, or to the graph that is being captured
-    ws = torch.empty(need.value, dtype=torch.uint8, device=device) if need.value else None
-    rc = _on_device(D.device, lambda stream: L.ms_custom_ops_chunk_attention(
-        C.byref(a), out_desc, lse_desc, None if ws is None else ws.data_ptr(), need.value, stream))
-    if rc:
-        _host.check(rc)
-    if fill or return_lse:
-        rows = int(np.sum(np.asarray(q_seq_lens), dtype=np.int64))
-        if rows < tokens:
-            if fill:
-                out[rows:].zero_()
-            if return_lse:
-                lse[rows:].fill_(-math.inf)
-    return (out, lse) if return_lse else out
+    r = _binding().chunk_attention(query, key_cache, value_cache, block_tables, _host_lens(q_seq_lens),
+                                   _host_lens(context_lens), qk_scale, window_size, input_layout, k_descale, k_offset,
+                                   v_descale, v_offset, out, return_lse, oob_count)
+    if r.__class__ is int:
+        _host.check(r)
+    return r if return_lse else r[0]
 
 
 def chunk_attention_infer(query, key_cache, value_cache, block_tables, q_seq_lens, context_lens, qk_scale=1.0,
@@ -697,7 +613,7 @@ def chunk_attention_infer(query, key_cache, value_cache, block_tables, q_seq_len
     D = _Descs()
     a = _chunk_args(_host.MsChunkAttentionArgs(), D, query, key_cache, value_cache, block_tables, q_seq_lens,
                     context_lens, qk_scale, window_size, input_layout, k_descale, k_offset, v_descale, v_offset,
-                    oob_count, {"host_ok": True})
+                    oob_count)
     dt, nd, shp = C.c_int32(), C.c_int32(), (C.c_int64 * _host.MS_MAX_DIMS)()
     _host.check(_host.lib().ms_custom_ops_chunk_attention_infer(C.byref(a), C.byref(dt), C.byref(nd), shp))
     return tuple(shp[i] for i in range(nd.value)), _DT_NAMES[dt.value]
@@ -709,8 +625,7 @@ def chunk_attention_workspace_size(query, key_cache, value_cache, block_tables, 
     """Bytes of device workspace a launch with these arguments needs (planning only, no GPU work)."""
     D = _Descs()
     a = _chunk_args(_host.MsChunkAttentionArgs(), D, query, key_cache, value_cache, block_tables, q_seq_lens,
-                    context_lens, qk_scale, window_size, input_layout, k_descale, k_offset, v_descale, v_offset, None,
-                    {"host_ok": True})
+                    context_lens, qk_scale, window_size, input_layout, k_descale, k_offset, v_descale, v_offset, None)
     n = C.c_size_t()
     _host.check(_host.lib().ms_custom_ops_chunk_attention_workspace_size(C.byref(a), C.byref(n)))
     return int(n.value)
@@ -743,18 +658,10 @@ def verify_draft_tokens(target_probs, draft_probs, draft_tokens, uniform, draft_
                  where the target is nowhere positive)
     accepted     int32 [batch]
     """
-    import torch
-    D = _packer(target_probs)
-    if draft_tokens.dim() != 2:
-        raise ValueError(f"For VerifyDraftTokens, draft_tokens must have rank 2, but got {draft_tokens.dim()}.")
-    batch, drafts = draft_tokens.shape
-    tokens = torch.empty((batch, drafts + 1), dtype=torch.int32, device=target_probs.device)
-    accepted = torch.empty((batch,), dtype=torch.int32, device=target_probs.device)
-    args = (D(target_probs), D(draft_probs), D(draft_tokens), D(uniform), D(draft_lens), D(tokens), D(accepted))
-    rc = _on_device(D.device, lambda stream: _host.lib().ms_custom_ops_verify_draft_tokens(*args, stream))
-    if rc:
-        _host.check(rc)
-    return tokens, accepted
+    r = _binding().verify_draft_tokens(target_probs, draft_probs, draft_tokens, uniform, draft_lens)
+    if r.__class__ is int:
+        _host.check(r)
+    return r
 
 
 def verify_draft_tokens_infer(target_probs, draft_probs, draft_tokens, uniform, draft_lens=None):

@@ -4,6 +4,7 @@
 
 libmsco_b200.so          CUDA kernels + thin C ABI      nvcc, sm_100a only
 libms_custom_ops_host.so C++ operator layer             g++, links the kernel library
+_torch_binding.so        Python binding (torch tensors) g++, links the operator layer and torch
 
 bench/msco_bench         standalone C++ benchmark       nvcc, links the kernel library
 
@@ -24,6 +25,8 @@ CSRC = os.path.join(HERE, "csrc")
 OPS = os.path.join(HERE, "ops")
 
 KERNEL_LIB = os.path.join(HERE, "libmsco_b200.so")
+BINDING_SRC = os.path.join(OPS, "binding", "torch_binding.cc")
+BINDING = os.path.join(HERE, "_torch_binding.so")
 HOST_LIB = os.path.join(HERE, "libms_custom_ops_host.so")
 
 NVCC_FLAGS = ["-std=c++17", "-O3", "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo",
@@ -63,7 +66,7 @@ def build_kernels(force=False, verbose_ptxas=False):
 
 
 def build_host(force=False):
-    srcs = sorted(glob.glob(os.path.join(OPS, "**", "*.cc"), recursive=True))
+    srcs = sorted(s for s in glob.glob(os.path.join(OPS, "**", "*.cc"), recursive=True) if s != BINDING_SRC)
     if not srcs:
         return None
     deps = srcs + glob.glob(os.path.join(OPS, "**", "*.h"), recursive=True) + glob.glob(os.path.join(INCLUDE, "*.h"))
@@ -73,6 +76,27 @@ def build_host(force=False):
            "-o", HOST_LIB] + srcs + ["-L", HERE, "-lmsco_b200", "-Wl,-rpath,$ORIGIN", "-lpthread"]
     _run(cmd)
     return HOST_LIB
+
+
+def build_binding(force=False):
+    """Python module that turns torch tensors into operator descriptors (ops/binding/torch_binding.cc)."""
+    deps = [BINDING_SRC] + glob.glob(os.path.join(INCLUDE, "*.h"))
+    if not force and not _stale(BINDING, deps):
+        return BINDING
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+    lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    cuda = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(_nvcc()))), "include")
+    inc = [INCLUDE, sysconfig.get_paths()["include"], cuda] + cpp_extension.include_paths()
+    cmd = ["g++", "-std=c++17", "-O2", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+    for i in inc:
+        cmd += ["-isystem" if i not in (INCLUDE,) else "-I", i]
+    cmd += ["-o", BINDING, BINDING_SRC, "-L", HERE, "-lms_custom_ops_host", "-lmsco_b200", "-Wl,-rpath,$ORIGIN", "-L", lib,
+            "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda"]
+    _run(cmd)
+    return BINDING
 
 
 def build_bench(force=False):
@@ -91,6 +115,7 @@ def build_bench(force=False):
 def build_all(force=False, verbose_ptxas=False):
     build_kernels(force, verbose_ptxas)
     build_host(force)
+    build_binding(force)
     build_bench(force)
 
 
