@@ -58,7 +58,7 @@ struct Cfg {
   static constexpr int kOffResp = (kOffBar + kNumBars * 8 + 16 + 15) / 16 * 16;  // answers of the launch control
   static constexpr int kOffPair = kOffResp + 32;               // [8] items of the softmax pairs
   static constexpr int kOffXch = kOffPair + 32;  // [stream][half][row]: what the two threads of a row exchange
-  static constexpr int kSmem = kOffXch + 2 * 2 * kRows * 4 + (KV8 ? kRows * 4 : 0);
+  static constexpr int kSmem = kOffXch + 2 * 2 * kRows * 4 + (KV8 ? (kRows + 32) * 4 : 0);
   // Of eight pairs of probabilities, those whose exponentials the FMA pipe computes.  At head_dim 128 the special-function
   // unit alone (1024 clocks a tile and stream) is as long as the two products: 2 of 8 took the prompt of 8192 tokens from
   // 503 to 460 us, 3 of 8 gave 475; at 64, where issue slots are short, any made it slower (316 us without, 355 with 2).
@@ -195,7 +195,8 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + C::kNumBars);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
   float *xch = reinterpret_cast<float *>(smem + C::kOffXch);
-  float *q_scale = xch + 2 * 2 * kRows;  // int8, single: what stream 0 found for the rows
+  float *q_scale = xch + 2 * 2 * kRows;  // int8, single: what stream 0 found for the rows, and for the first 32
+  float *q_shift = q_scale + kRows;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (threadIdx.x == 0) {
@@ -645,6 +646,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           sc = p.scale_log2e / up;
           shift = off * p.scale_log2e;
           if (!w.dual && hf == 0) q_scale[row] = sc;
+          if (!w.dual && hf == 0 && row < 32) q_shift[row] = shift;
           fence_proxy_async();
         }
         __syncwarp();
@@ -758,6 +760,61 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         l += *x_other;
       }
       const bool two = !w.dual && w.n > 1;  // two states of the same rows
+      const bool split = e.nsplit > 1;
+      const int tile_rows = min(p.item_tokens, e.q_len) * g;
+      const int64_t part_row0 = (int64_t)e.part_base +
+                                ((int64_t)(w.it.qtile * e.nsplit + w.it.split) * p.num_kv_heads + w.it.kvh) * tile_rows;
+      if (two && ntok * g <= 32) {
+        // Up to 32 rows (one warp of each half has them): both streams lay all their columns down, [stream][column][row], and
+        // all 512 threads add and write eight columns of a row each.  Row by row, as below, this took 7000 clocks of an
+        // item that reads its four tiles in 11000.
+        float *buf = reinterpret_cast<float *>(smem + C::kQBytes);
+        if (warp_live) {
+          pair_sync();  // the sums have been read
+          *x_mine = hf == 0 ? m : l;
+#pragma unroll 1
+          for (int c = 0; c < D / 2; c += 32) {
+            uint32_t o[32];
+            tmem_ld32(t_o + c, o);
+            tmem_wait_ld32(o);
+            float *dst = buf + (s * D + hf * (D / 2) + c) * 32 + lane;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) dst[i * 32] = __uint_as_float(o[i]);
+          }
+        }
+        tc_fence_before();
+        merge_sync();
+        const int rows = ntok * g, n = (int)threadIdx.x - C::kFirstSoft * 32;
+        const int rr = n % rows, c0 = n / rows * 8;
+        if (c0 < D) {
+          const float m0 = xch[rr], l0 = xch[kRows + rr], m1 = xch[2 * kRows + rr], l1 = xch[3 * kRows + rr];
+          const float mm = fmaxf(m0, m1), b = mm == -INFINITY ? 0.f : mm;
+          const float f0 = fast_exp2(m0 - b), f1 = fast_exp2(m1 - b), ll = l0 * f0 + l1 * f1;
+          uint32_t o[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            o[i] = __float_as_uint(buf[(c0 + i) * 32 + rr] * f0 + buf[(D + c0 + i) * 32 + rr] * f1);
+          const int64_t orow2 = ((int64_t)e.q_start + tok0 + rr / g) * p.num_q_heads + w.it.kvh * g + rr % g;
+          const float m_row = mm + (KV8 ? q_shift[rr] : 0.f);
+          if (split) {
+            store_32b(p.part_o + (part_row0 + rr) * D + c0, o);
+            if (c0 == 0) *reinterpret_cast<float2 *>(p.part_ml + (part_row0 + rr) * 2) = make_float2(m_row, ll);
+          } else {
+            const float inv2 = ll > 0.f ? 1.f / ll : 0.f;
+            float f[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              f[i] = __uint_as_float(o[i]) * inv2;
+              if (KV8) f[i] = dequant_out(p, w.it.kvh * D + c0 + i, f[i], inv2);
+            }
+            *reinterpret_cast<uint4 *>(static_cast<T *>(p.out) + orow2 * D + c0) =
+                make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
+            if (c0 == 0 && p.lse != nullptr) p.lse[orow2] = ll > 0.f ? (m_row + log2f(ll)) * kLn2 : -INFINITY;
+          }
+        }
+        fence_proxy_async();  // the buffer's next use is by the loads
+        merge_sync();
+      } else {
       float scale0 = 1.f, scale1 = 0.f, m_out = m, l_out = l;
       if (two) {
         if (s == 1) {
@@ -776,11 +833,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       }
       const int64_t tok = (int64_t)e.q_start + tok0 + tok_in;
       const int64_t orow = tok * p.num_q_heads + w.it.kvh * g + head_in;
-      const bool split = e.nsplit > 1;
-      const int tile_rows = min(p.item_tokens, e.q_len) * g;
-      const int64_t prow = (int64_t)e.part_base +
-                           ((int64_t)(w.it.qtile * e.nsplit + w.it.split) * p.num_kv_heads + w.it.kvh) * tile_rows +
-                           (tok0 - w.it.tok0) * g + row;
+      const int64_t prow = part_row0 + (tok0 - w.it.tok0) * g + row;
       const float inv = split ? 1.f : (l_out > 0.f ? 1.f / l_out : 0.f);
       const bool writes = live && (w.dual || s == 0);
       // This half's columns that go through the merge buffer (the space of Q's second tile) at a time: with up to 64 rows
@@ -840,13 +893,14 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           merge_sync();
         }
       }
-      // the merge buffer lies over Q's second tile: only now may the next item's rows come in
-      if (!KV8 && speaker && w.n > 0 && !w.dual && lane == 0) mbar_arrive(&m_free[k_item & 1]);
       if (writes && hf == 0) {
         m_out += shift;
         if (split) *reinterpret_cast<float2 *>(p.part_ml + prow * 2) = make_float2(m_out, l_out);
         else if (p.lse != nullptr) p.lse[orow] = l_out > 0.f ? (m_out + log2f(l_out)) * kLn2 : -INFINITY;
       }
+      }
+      // the merge buffer lies over Q's second tile: only now may the next item's rows come in
+      if (!KV8 && speaker && w.n > 0 && !w.dual && lane == 0) mbar_arrive(&m_free[k_item & 1]);
       tc_fence_before();  // the reads of O are ordered before the next item's products (which wait for its P)
       if (hf == 0) {
         const bool more = it.next(wait, lane);
