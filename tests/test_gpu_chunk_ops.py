@@ -230,6 +230,35 @@ def test_long_contexts(q_lens, ctx, dim):
     Chunk(q_lens, ctx, heads=8, kv_heads=2, dim=dim, block=128, seed=sum(ctx)).check()
 
 
+@pytest.mark.parametrize("window", [700, 5000])
+def test_windows_over_long_contexts(window):
+    Chunk([1, 3, 200, 1], [20000, 9000, 15000, 130], heads=8, kv_heads=2, block=64, window=window, seed=window).check()
+    Chunk([129, 1], [9000, 12001], heads=2, kv_heads=2, dim=64, block=16, window=window, seed=window).check()
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(8, 2), (8, 8), (40, 1), (64, 2)])
+@pytest.mark.parametrize("offsets", [False, True])
+def test_few_rows_over_long_int8_contexts(heads, kv_heads, offsets):
+    Chunk([4, 1, 2, 1], [9000, 20000, 131, 128], heads=heads, kv_heads=kv_heads, block=128, int8=True, offsets=offsets,
+          seed=heads).check()
+
+
+@pytest.mark.parametrize("which", ["query", "out"])
+def test_rows_that_are_not_aligned(which):
+    # copies of 16 bytes cannot start on them: the general kernel takes the call
+    c = Chunk([20, 1], [300, 1000], block=16, seed=33)
+    base = torch.empty(c.query.numel() + 1, dtype=c.query.dtype, device="cuda")
+    view = base[1:].view(c.query.shape)
+    if which == "query":
+        view.copy_(c.query)
+        c.query = view
+        c.check()
+    else:
+        out, lse = c.run(out=view, return_lse=True)
+        assert out is view
+        c.check(out, lse)
+
+
 def test_large_scores_and_negative_scale():
     c = Chunk([100], [400], dtype="fp16", scale=3.0, seed=5)
     c.check()
