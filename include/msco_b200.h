@@ -467,8 +467,9 @@ int msco_rope_and_cache(const MscoRopeDesc *desc, const void *query, const void 
  *   lse          float32 [tokens, num_q_heads] or NULL
  * Lengths are read on the host during the call; nothing of them is kept.  Block ids outside the cache are read
  * as block 0 and counted in *oob_count (device int32, may be NULL).  Cached tokens that no query of the chunk
- * may see are not read, or do not count whatever they hold.  The result of a sequence does not depend on
- * the other sequences of the call.
+ * may see are not read, or do not count whatever they hold; a value that is not finite in a token that some query
+ * of the chunk sees may reach the others of that sequence's chunk too (its weight there is 0, and 0 * inf is NaN).
+ * The result of a sequence does not depend on the other sequences of the call.
  * `workspace`: 256-byte aligned device memory of msco_chunk_attention_workspace bytes (may be 0), not
  * shared with a call in flight; it needs no initialisation.
  * ---------------------------------------------------------------------- */

@@ -596,6 +596,8 @@ def chunk_attention(query, key_cache, value_cache, block_tables, q_seq_lens, con
     oob_count    int32 [1] or None: incremented for every block id outside the cache that was met (such a block
                  is read as block 0)
     The i-th of q_len new tokens stands at position context_len - q_len + i; one that sees nothing gives zeros.
+    What the caches hold outside the tokens that the chunk sees does not matter; a key or value among them that is not
+    finite may reach every new token of its sequence.  A batch of single tokens alone is ``paged_attention``'s case.
     The lengths are read during the call: a captured graph replays with the lengths it was captured with.
     """
     r = _binding().chunk_attention(query, key_cache, value_cache, block_tables, _host_lens(q_seq_lens),

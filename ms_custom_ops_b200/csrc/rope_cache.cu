@@ -165,12 +165,16 @@ __global__ void __launch_bounds__(256) rope_cache_vec_kernel(RopeArgs a) {
   const int32_t *of = kind == 1 ? a.k_offset : a.v_offset;
   auto put8 = [&](int i, const float (&y)[8]) {  // quantised row i
     const int c = (h0 + i) * D;
-    uint32_t q8[2] = {0, 0};
+    uint32_t q8[2];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const int d = k < 4 ? d0 + k : d1 + k - 4;
-      q8[k / 4] |= (uint32_t)(uint8_t)quantise(y[k], __ldg(ds + c + d), of != nullptr ? (float)__ldg(of + c + d) : 0.f)
-                   << (8 * (k & 3));
+    for (int n = 0; n < 2; ++n) {
+      const int d = c + (n == 0 ? d0 : d1);
+      const float4 s4 = __ldg(reinterpret_cast<const float4 *>(ds + d));
+      const int4 o4 = of != nullptr ? __ldg(reinterpret_cast<const int4 *>(of + d)) : make_int4(0, 0, 0, 0);
+      q8[n] = (uint32_t)(uint8_t)quantise(y[4 * n], s4.x, (float)o4.x) |
+              (uint32_t)(uint8_t)quantise(y[4 * n + 1], s4.y, (float)o4.y) << 8 |
+              (uint32_t)(uint8_t)quantise(y[4 * n + 2], s4.z, (float)o4.z) << 16 |
+              (uint32_t)(uint8_t)quantise(y[4 * n + 3], s4.w, (float)o4.w) << 24;
     }
     *reinterpret_cast<uint32_t *>(dst8 + i * step + d0) = q8[0];
     *reinterpret_cast<uint32_t *>(dst8 + i * step + d1) = q8[1];
@@ -303,7 +307,9 @@ int launch_rope(const RopeArgs &a, cudaStream_t st) {
   const uintptr_t all = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) |
                         reinterpret_cast<uintptr_t>(a.q_out) | reinterpret_cast<uintptr_t>(a.k_cache) |
                         reinterpret_cast<uintptr_t>(a.v_cache) | reinterpret_cast<uintptr_t>(a.cos_sin) |
-                        reinterpret_cast<uintptr_t>(a.q_weight) | reinterpret_cast<uintptr_t>(a.k_weight);
+                        reinterpret_cast<uintptr_t>(a.q_weight) | reinterpret_cast<uintptr_t>(a.k_weight) |
+                        reinterpret_cast<uintptr_t>(a.k_descale) | reinterpret_cast<uintptr_t>(a.v_descale) |
+                        reinterpret_cast<uintptr_t>(a.k_offset) | reinterpret_cast<uintptr_t>(a.v_offset);
   const bool strides = a.tokens == 1 || ((a.q_stride | a.k_stride | a.v_stride) & 7) == 0;
   const bool vec = (all & 15) == 0 && strides && a.rotary % (a.interleaved ? 8 : 16) == 0;
   if (vec && a.head_dim == 128) return launch_vec_of<T, 128, I8>(a, st);
